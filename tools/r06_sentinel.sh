@@ -1,9 +1,8 @@
 #!/bin/bash
-# Round 6: the range sentinel on the box -- scalar-store probe, the range tests, and a same-box A/B of the S1 step with the probes on / off
+# Round 6: the range sentinel on the box -- the range tests, and a same-box A/B of the S1 step with the probes on / off
 cd /tmp && export TMPDIR=/tmp && cd $GRAFT_REPO_ROOT
 export GPU_MAX_HW_QUEUES=8
 O=gpurun_out/r6sent; mkdir -p $O
-./tools/probes/bin/sstore_probe > $O/sstore_probe.txt 2>&1; cat $O/sstore_probe.txt
 timeout 1500 python -m pytest tests/test_gpu_range.py -x -q -s 2>&1 | tail -60 > $O/range_tests.txt; tail -40 $O/range_tests.txt
 P="--in-flight 0 --no-cpu-baseline --no-train --no-exact-pass --no-attn-phase"
 for rep in 1 2; do

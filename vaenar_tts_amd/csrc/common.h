@@ -159,15 +159,18 @@ typedef _Float16 vnr_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 vnr_h8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ void vnr_split(const vnr_f4 x, vnr_h4& hi, vnr_h4& lo) {
   hi = __builtin_convertvector(x, vnr_h4);
+  asm("" : "+v"(hi));          // one value for both uses: without packed fp32 the elements' conversions would be folded into the arithmetic again
   lo = __builtin_convertvector(x - __builtin_convertvector(hi, vnr_f4), vnr_h4);
 }
 __device__ __forceinline__ void vnr_split(const vnr_f8 x, vnr_h8& hi, vnr_h8& lo) {
   hi = __builtin_convertvector(x, vnr_h8);
+  asm("" : "+v"(hi));
   lo = __builtin_convertvector(x - __builtin_convertvector(hi, vnr_f8), vnr_h8);
 }
 __device__ __forceinline__ void vnr_split(const float x, _Float16& hi, _Float16& lo) {      // one value: the same conversion on a pair
   const vnr_f2 xv = {x, x};
-  const vnr_h2 h = __builtin_convertvector(xv, vnr_h2);
+  vnr_h2 h = __builtin_convertvector(xv, vnr_h2);
+  asm("" : "+v"(h));
   const vnr_h2 l = __builtin_convertvector(xv - __builtin_convertvector(h, vnr_f2), vnr_h2);
   hi = h[0]; lo = l[0];
 }
@@ -282,14 +285,20 @@ constexpr int kMaxChainStages = 20;
 // NaN, whatever the weights -- and an activation function may heal it on the way out (fmaxf(NaN, 0) = 0: a ReLU stage would hand on
 // zeros).  Each split product therefore looks at ONE accumulator per row right behind its k-loop and raises the handle's flag word
 // (host-pinned: the engine reads it at its synchronisation points, engine.hip "range sentinel").  Rare branch, no state kept.
-__device__ __forceinline__ void range_note(unsigned* flag, float acc_elem) {
+__device__ __forceinline__ void range_note(unsigned* flag, float& acc_elem) {
   const bool bad = !(__builtin_fabsf(acc_elem) < __builtin_inff());
-  // wave-uniform branch + SCALAR store (s_store_dword exists on the gfx9 family; tools/probes/sstore_probe.hip): the raise needs no vector
-  // register -- with a vector store the one-wave-per-SIMD chain kernel (512 registers in use) spilled.  `flag` is never null (an unwatched
-  // launch gets the handle's scrap word): a null test in front would keep the pointer live across the kernel's stage loop.
+  // wave-uniform branch + a vector store that needs NO vector register of its own: the one-wave-per-SIMD chain kernel (512 registers in use)
+  // has none (an address pair and a value made it spill).  One lane lends the probed element's register: its value waits in a scalar
+  // register, the register holds 1 -- the value to store, and the offset that the instruction's -1 takes back from the scalar address --
+  // and gets its value back once the store has left.  `flag` is never null (an unwatched launch gets the handle's scrap word): a null test
+  // in front would keep the pointer live across the kernel's stage loop.  sc0 sc1: past the caches, the host reads the word behind a
+  // synchronisation.  (s_nop: the pair may come from a lane read, five wait states in front of its use as an address.)
   if (__builtin_amdgcn_ballot_w64(bad)) {
-    const unsigned one = 1u;
-    asm volatile("s_store_dword %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::"s"(one), "s"(flag) : "memory");
+    unsigned lane, keep;
+    asm volatile("s_mov_b64 vcc, exec\n\ts_ff1_i32_b64 %1, exec\n\tv_readfirstlane_b32 %2, %0\n\ts_mov_b64 exec, 0\n\ts_bitset1_b64 exec, %1\n\t"
+                 "s_nop 0\n\tv_mov_b32 %0, 1\n\ts_nop 4\n\tglobal_store_dword %0, %0, %3 offset:-1 sc0 sc1\n\ts_waitcnt vmcnt(0)\n\t"
+                 "v_mov_b32 %0, %2\n\ts_mov_b64 exec, vcc"
+                 : "+v"(acc_elem), "=&s"(lane), "=&s"(keep) : "s"(flag) : "vcc", "memory");
   }
 }
 __device__ __forceinline__ void out_store4(float* p, float a, float b, float c, float d) {

@@ -74,6 +74,14 @@ __device__ __forceinline__ void panel_put4(char* P, int r, int kt, int p, const 
 }
 }  // namespace
 
+// The lane's number, counted anew where it is asked for: no register carries it there (this kernel has none to spare; a copy kept
+// across the stages is one the compiler spills)
+__device__ __forceinline__ int lane_now() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+
 __global__ void __launch_bounds__(256)
 panel_chain4_kernel(const ChainArgs g) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -121,7 +129,7 @@ panel_chain4_kernel(const ChainArgs g) {
     frs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(w), 0, 0x40000000, 0x00020000);
     fnk = nk;
     fpad = (nk + kDepth - 1) / kDepth * kDepth;
-    fvoff0 = (64 * wave < n) ? (unsigned)(((2 * wave) * ktt + k0) * 4096 + lane * 16) : kOob3;
+    fvoff0 = (64 * wave < n) ? (unsigned)(((2 * wave) * ktt + k0) * 4096 + lane_now() * 16) : kOob3;
     fjd = ktt * 4096;
     fj1 = 64 * wave + 32 < n;
   };
@@ -293,13 +301,10 @@ panel_chain4_kernel(const ChainArgs g) {
 
 #pragma unroll 1
   for (int si = 0; si < g.nstages; ++si) {
-    // every lane-dependent address of a stage is re-derived from an opaque copy of the lane id (gemm3.hip: otherwise the compiler
+    // every lane-dependent address of a stage is re-derived from a lane id counted anew (gemm3.hip: otherwise the compiler
     // hoists dozens of loop-invariant offsets out of the stage loop and spills them)
-    int lane_s = lane;
-    asm volatile("" : "+v"(lane_s));
+    const int lane_s = lane_now();
     const int half = lane_s >> 5, l31 = lane_s & 31;
-    int tid_s = tid;
-    asm volatile("" : "+v"(tid_s));
     if (tid == 0) chain_publish_stage(g, si);               // (chain_prefetch.h)
     if (ts && tid == 0) ts[96 + si] = __builtin_amdgcn_s_memrealtime();      // (measurement: 100 MHz, the same clock on every CU)
     if (g.att_stage > 0 && si == g.att_stage) {
@@ -603,6 +608,7 @@ panel_chain4_kernel(const ChainArgs g) {
     if (vstage) {
       if (wave_on) {
         // both 32 x 32 blocks of the wave at once (two wave-private [32 channels][33] float buffers): all writes, ONE wait, all reads
+        const int l31v = lane_now() & 31;
         const int Hh = st.aoi_D >> 6, TT = (st.aoi_T + 31) >> 5;
         float* tb = reinterpret_cast<float*>(smem + g.vt_lds) + wave * (2 * 32 * 33);
         const float* bp = prm + si * 256 + 64 * wave;                   // (zero padded when the stage has no bias)
@@ -620,9 +626,9 @@ panel_chain4_kernel(const ChainArgs g) {
             const float bq[4] = {bi[j][q].x, bi[j][q].y, bi[j][q].z, bi[j][q].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float tv = acc[j][4 * q + e] * st.scale + bq[e];
+              float tv = acc[j][4 * q + e] * st.scale + bq[e];
               if (j == 0 && q == 0 && e == 0) range_note(g.range_flag, tv);
-              tb[j * (32 * 33) + (8 * q + 4 * half + e) * 33 + l31] = tv;
+              tb[j * (32 * 33) + (8 * q + 4 * half + e) * 33 + l31v] = tv;
             }
           }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -633,12 +639,12 @@ panel_chain4_kernel(const ChainArgs g) {
 #pragma unroll
           for (int tp = 0; tp < 2; ++tp)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[j][tp][e] = tb[j * (32 * 33) + l31 * 33 + 16 * tp + (e & 3) + 4 * half + 8 * (e >> 2)];   // k-slot (tp, g = half, e) -> row of the panel
+            for (int e = 0; e < 8; ++e) x[j][tp][e] = tb[j * (32 * 33) + l31v * 33 + 16 * tp + (e & 3) + 4 * half + 8 * (e >> 2)];   // k-slot (tp, g = half, e) -> row of the panel
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (j == 1 && !j1) continue;
-          const int cv = st.aoi_c0 - 2 * st.aoi_D + 32 * (2 * wave + j) + l31;   // V column of this lane: head cv >> 6, channel cv & 63
+          const int cv = st.aoi_c0 - 2 * st.aoi_D + 32 * (2 * wave + j) + l31v;   // V column of this lane: head cv >> 6, channel cv & 63
 #pragma unroll
           for (int tp = 0; tp < 2; ++tp) {
             const int R = m0 + 16 * tp;
@@ -650,7 +656,7 @@ panel_chain4_kernel(const ChainArgs g) {
             for (int e = 0; e < 8; ++e) x8[e] = x[j][tp][e];
             split_hi_lo(x8, hi, lo);
             char* pdst = reinterpret_cast<char*>(st.out) + 2 * st.aoi_img_bytes + ((size_t)(bb * Hh + (cv >> 6)) * TT + (tt >> 5)) * kAoiTile +
-                         ((tt >> 4) & 1) * 2048 + ((cv >> 5) & 1) * 1024 + ((half * 32 + l31) << 4);
+                         ((tt >> 4) & 1) * 2048 + ((cv >> 5) & 1) * 1024 + ((half * 32 + l31v) << 4);
             *reinterpret_cast<h16x8*>(pdst) = hi;
             *reinterpret_cast<h16x8*>(pdst + 4096) = lo;
           }
@@ -835,8 +841,9 @@ panel_chain4_kernel(const ChainArgs g) {
       wstamp(si, 7);
       if (half == 0) { scratch[l31 * 4 + wave] = s1; scratch[kRows * 4 + l31 * 4 + wave] = m2; }
       lds_barrier4();                                                   // (also: every wave is done reading the source / residual panels)
-      const f32x4 sa = *reinterpret_cast<const f32x4*>(scratch + l31 * 4);
-      const f32x4 ma = *reinterpret_cast<const f32x4*>(scratch + kRows * 4 + l31 * 4);
+      const int l31n = lane_now() & 31;
+      const f32x4 sa = *reinterpret_cast<const f32x4*>(scratch + l31n * 4);
+      const f32x4 ma = *reinterpret_cast<const f32x4*>(scratch + kRows * 4 + l31n * 4);
       const float mu = (sa[0] + sa[1] + sa[2] + sa[3]) * (1.f / 256.f);
       float var = 0.f;
 #pragma unroll
@@ -862,8 +869,8 @@ panel_chain4_kernel(const ChainArgs g) {
           *reinterpret_cast<h16x4*>(Dp + po[j][q]) = xh[j][q];
           *reinterpret_cast<h16x4*>(Dp + (po[j][q] ^ 64)) = xl[j][q];
         }
-      if (st.out && m0 + l31 < mend) {
-        float* orow = st.out + (size_t)(m0 + l31) * st.ldo + 64 * wave + 4 * half;
+      if (st.out && m0 + l31n < mend) {
+        float* orow = st.out + (size_t)(m0 + l31n) * st.ldo + 64 * wave + 4 * half;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -893,6 +900,7 @@ panel_chain4_kernel(const ChainArgs g) {
         v[j][4 * q + 3] = acc[j][4 * q + 3] * st.scale + bi.w;
       }
     range_note(g.range_flag, v[0][0]);
+    const int l31e = lane_now() & 31;
     if (st.act == ACT_RELU) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -917,18 +925,19 @@ panel_chain4_kernel(const ChainArgs g) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (cok[j][q])
-              *reinterpret_cast<float4*>(cx + l31 * cst + 32 * (2 * wave + j) + 8 * q + 4 * half) =
+              *reinterpret_cast<float4*>(cx + l31e * cst + 32 * (2 * wave + j) + 8 * q + 4 * half) =
                   make_float4(v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
       }
       // the four pieces of z this thread works on are requested BEFORE the exchange barrier (they do not depend on the heads): one memory
       // round trip under the barrier instead of four behind it
-      const int c = (tid_s & 15) * 4;
+      const int tid_n = 64 * wave + lane_now();
+      const int c = (tid_n & 15) * 4;
       float4 zo[2][2];
 #pragma unroll
       for (int rr = 0; rr < 2; ++rr)
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
-          const int row = m0 + 16 * rr + (tid_s >> 4);
+          const int row = m0 + 16 * rr + (tid_n >> 4);
           zo[rr][which] = row < mend ? *reinterpret_cast<const float4*>(g.cpl_z + (size_t)row * g.cpl_ld + (which ? g.cpl_cond_off : g.cpl_zp_off) + c)
                                      : make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -937,7 +946,7 @@ panel_chain4_kernel(const ChainArgs g) {
         char* Dp = panel_ptr(st.dst);
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
-          const int prow = 16 * rr + (tid_s >> 4), row = m0 + prow;
+          const int prow = 16 * rr + (tid_n >> 4), row = m0 + prow;
 #pragma unroll
           for (int which = 0; which < 2; ++which) {
             const int zoff = which ? g.cpl_cond_off : g.cpl_zp_off;
@@ -962,7 +971,7 @@ panel_chain4_kernel(const ChainArgs g) {
       continue;
     }
     {
-      const int row = m0 + l31;
+      const int row = m0 + l31e;
       if (st.pe) {                                                      // + pos_weight * PE[t] (encoder.py:85, transform.py:51)
         const float* pr = st.pe + (size_t)(row % st.pe_T) * st.n;
 #pragma unroll
@@ -983,8 +992,8 @@ panel_chain4_kernel(const ChainArgs g) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int kt = 2 * wave + j, p = 8 * q + 4 * half;
-            const h16x4 rh = *reinterpret_cast<const h16x4*>(Rp + panel_off4(l31, kt, p >> 3) + (p & 4) * 2);
-            const h16x4 rl = *reinterpret_cast<const h16x4*>(Rp + panel_off4(l31, kt, 4 + (p >> 3)) + (p & 4) * 2);
+            const h16x4 rh = *reinterpret_cast<const h16x4*>(Rp + panel_off4(l31e, kt, p >> 3) + (p & 4) * 2);
+            const h16x4 rl = *reinterpret_cast<const h16x4*>(Rp + panel_off4(l31e, kt, 4 + (p >> 3)) + (p & 4) * 2);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[j][4 * q + e] += (float)rh[e] + (float)rl[e];
           }
@@ -997,7 +1006,7 @@ panel_chain4_kernel(const ChainArgs g) {
     }
     wstamp(si, 6);                                       // (finer epilogue stamps, measurement) residual / PE added
     if (st.gamma && st.out_pre) {                                       // training: x + Dense(.) before the normalisation
-      const int row = m0 + l31;
+      const int row = m0 + l31e;
       if (row < mend) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -1030,12 +1039,12 @@ panel_chain4_kernel(const ChainArgs g) {
           }
       m2 += __shfl_xor(m2, 32, 64);
       wstamp(si, 7);                                     // row statistics of this wave's columns ready
-      if (half == 0) { scratch[l31 * 4 + wave] = s1; scratch[kRows * 4 + l31 * 4 + wave] = m2; }
+      if (half == 0) { scratch[l31e * 4 + wave] = s1; scratch[kRows * 4 + l31e * 4 + wave] = m2; }
       lds_barrier4();
       const float* lnp = prm + st.lds_ln;                               // gamma [256] | beta [256]
       const float rn = 1.f / (float)st.n;
-      const f32x4 sa = *reinterpret_cast<const f32x4*>(scratch + l31 * 4);
-      const f32x4 ma = *reinterpret_cast<const f32x4*>(scratch + kRows * 4 + l31 * 4);
+      const f32x4 sa = *reinterpret_cast<const f32x4*>(scratch + l31e * 4);
+      const f32x4 ma = *reinterpret_cast<const f32x4*>(scratch + kRows * 4 + l31e * 4);
       const float tot = sa[0] + sa[1] + sa[2] + sa[3];
       const float mu = tot * rn;
       float var = 0.f;
@@ -1046,8 +1055,8 @@ panel_chain4_kernel(const ChainArgs g) {
         var += ma[w] + (float)c * dm * dm;
       }
       const float rstd = 1.0f / sqrtf(var * rn + kLnEps);
-      if (st.out_stats && wave == 0 && half == 0 && m0 + l31 < mend)
-        *reinterpret_cast<float2*>(st.out_stats + 2 * (size_t)(m0 + l31)) = make_float2(mu, rstd);
+      if (st.out_stats && wave == 0 && half == 0 && m0 + l31e < mend)
+        *reinterpret_cast<float2*>(st.out_stats + 2 * (size_t)(m0 + l31e)) = make_float2(mu, rstd);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -1065,7 +1074,7 @@ panel_chain4_kernel(const ChainArgs g) {
     wstamp(si, 2);
     // ---- outputs: HBM (fp32, 16-byte row pieces) and/or destination panel (split fp16) -----------------------------------
     {
-      const int row = m0 + l31;
+      const int row = m0 + l31e;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int cb = 32 * (2 * wave + j);                             // first column of this block
@@ -1103,7 +1112,7 @@ panel_chain4_kernel(const ChainArgs g) {
             }
             else out_store4(st.out + (size_t)row * st.ldo + col, v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3]);
           }
-          if (st.dst >= 0) panel_put4(panel_ptr(st.dst), l31, col >> 5, col & 31, &v[j][4 * q]);
+          if (st.dst >= 0) panel_put4(panel_ptr(st.dst), l31e, col >> 5, col & 31, &v[j][4 * q]);
         }
       }
     }

@@ -1162,6 +1162,8 @@ attn_bwd_dkv_mfma_kernel(const AttnBwdArgs a, const unsigned* amax) {
         const float4 g0 = ok ? *reinterpret_cast<const float4*>(qp) : make_float4(0.f, 0.f, 0.f, 0.f), g1 = ok ? *reinterpret_cast<const float4*>(qp + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
         x[0] = d0.x * sc; x[1] = d0.y * sc; x[2] = d0.z * sc; x[3] = d0.w * sc; x[4] = d1.x * sc; x[5] = d1.y * sc; x[6] = d1.z * sc; x[7] = d1.w * sc;
         y[0] = g0.x; y[1] = g0.y; y[2] = g0.z; y[3] = g0.w; y[4] = g1.x; y[5] = g1.y; y[6] = g1.z; y[7] = g1.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) asm("" : "+v"(x[e]));          // the scaled value is formed once, in fp32: the split subtracts from what it rounds
         h16x8_t xh, xl, yh, yl;
         split8_t(x, xh, xl);
         split8_t(y, yh, yl);
@@ -1228,6 +1230,8 @@ attn_bwd_dkv_mfma_kernel(const AttnBwdArgs a, const unsigned* amax) {
         const float4 g0 = ok ? *reinterpret_cast<const float4*>(qp) : make_float4(0.f, 0.f, 0.f, 0.f), g1 = ok ? *reinterpret_cast<const float4*>(qp + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
         x[0] = d0.x * sc; x[1] = d0.y * sc; x[2] = d0.z * sc; x[3] = d0.w * sc; x[4] = d1.x * sc; x[5] = d1.y * sc; x[6] = d1.z * sc; x[7] = d1.w * sc;
         y[0] = g0.x; y[1] = g0.y; y[2] = g0.z; y[3] = g0.w; y[4] = g1.x; y[5] = g1.y; y[6] = g1.z; y[7] = g1.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) asm("" : "+v"(x[e]));          // the scaled value is formed once, in fp32: the split subtracts from what it rounds
         h16x8_t xh, xl, yh, yl;
         split8_t(x, xh, xl);
         split8_t(y, yh, yl);
