@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define VNR_ABI_VERSION 6
+#define VNR_ABI_VERSION 7
 
 typedef struct vnr_context *vnr_handle;
 
@@ -249,6 +249,75 @@ int vnr_op_kernel_grad(vnr_handle h, const float *d_x, int ldx, const float *d_d
 int vnr_random_normal(vnr_handle h, uint64_t seed, uint64_t offset, float stddev, float *d_out, size_t n);
 /* PositionalEncoding.positional_encoding (modules/utils.py:333-355): d_out [T,dim]. */
 int vnr_op_positional_encoding(vnr_handle h, int T, int dim, float step, float *d_out);
+
+/* ---- operators on packed sequences and on a paged key / value cache ---------------------------------------------------------------
+ * Ragged batches without their padding: the rows of all sequences lie one behind the other in [rows][heads][head_dim] matrices (a row
+ * stride in ELEMENTS may leave room between rows: column blocks of one projection), sequence b owning rows d_cu[b] .. d_cu[b + 1] - 1
+ * (device int32 [batch + 1], ascending).  Query head h reads key / value head h / (heads / kv_heads).  Types: every tensor of a call in the
+ * same one of the three; products are rounded once (16 bits: the probabilities and their gradients as operands of the second products),
+ * maxima, sums and accumulators are 32 bits.  head_dim: a multiple of 8, at most 128.  Matrices: 16-byte aligned, row strides a multiple
+ * of 16 bytes.  scale > 0.  Outputs must not overlap inputs.  Rows outside d_cu[0] .. d_cu[batch] - 1 are neither read nor written, and a
+ * masked or absent key contributes nothing whatever it holds (infinities and NaN included) -- see vnr_op_packed_attention_grad for its
+ * exception.  Starts that run backwards or leave the tensor make a sequence empty; nothing outside a tensor is touched.  Refused calls
+ * return VNR_ERR_ARG with a message and launch nothing.  All calls are asynchronous on the handle's stream, which is not any other
+ * library's: memory that another stream writes has to be complete before the call. */
+enum { VNR_F32 = 0, VNR_F16 = 1, VNR_BF16 = 2 };
+typedef struct vnr_packed_attention_desc {
+  int32_t dtype, batch, heads, kv_heads, head_dim;
+  int32_t causal;                          /* 1: row i of a sequence of nq rows and nk keys sees keys 0 .. i + nk - nq (the last row sees all); 0: all nk */
+  float   scale;
+  int32_t rows_q, rows_k;                  /* rows of the matrices */
+  const int32_t *d_cu_q, *d_cu_k;          /* [batch + 1]; the same array where queries and keys come from the same rows */
+  const void *d_q, *d_k, *d_v;             /* [rows_q][heads][head_dim], [rows_k][kv_heads][head_dim] */
+  int64_t ldq, ldk, ldv;
+  void *d_out; int64_t ldo;                /* [rows_q][heads][head_dim] */
+  float *d_lse;                            /* [heads][rows_q]: log of the row's sum of exponentials (natural); NULL where it is not wanted */
+} vnr_packed_attention_desc;
+typedef struct vnr_packed_attention_grad {
+  const void *d_dout; int64_t lddo;        /* gradient of d_out */
+  void *d_dq, *d_dk, *d_dv;                /* written in full for every row of a sequence */
+  int64_t lddq, lddk, lddv;
+} vnr_packed_attention_grad;
+/* out = softmax(scale q k' + mask) v of every sequence (MultiHeadScaledProductAttention.call, modules/attention.py:224-246, without its
+ * padding).  A row that sees no key: zeros, d_lse = -infinity. */
+int vnr_op_packed_attention(vnr_handle h, const vnr_packed_attention_desc *desc);
+/* Its gradient, from the forward's d_out and d_lse.  No atomics: the same bits every time.  Rows and keys that see nothing get zeros. */
+int vnr_op_packed_attention_grad(vnr_handle h, const vnr_packed_attention_desc *desc, const vnr_packed_attention_grad *grad);
+
+/* Pools of pages, [pages][kv_heads][page_size][head_dim] each; position p of sequence b lives in page d_table[b][p / page_size].
+ * page_size: a power of two, at most 4096. */
+typedef struct vnr_kv_cache {
+  int32_t dtype, kv_heads, head_dim, pages, page_size;
+  void *d_k, *d_v;
+} vnr_kv_cache;
+/* d_table[i][c] = cos, d_table[i][rot_dim / 2 + c] = sin of i / base^(2 c / rot_dim), i < positions: from 64 bits, rounded once */
+int vnr_op_rotation_table(vnr_handle h, int positions, int rot_dim, double base, float *d_table);
+/* New keys and values of a batch into the cache: row d_cu[b] + i goes to position d_context[b] + i of sequence b.  The first rot_dim
+ * channels of a key turn by their position on the way (channel c with c + rot_dim / 2, or with interleaved = 1 channel 2 c with 2 c + 1);
+ * rot_dim = 0: no rotation.  With d_q the queries of the same rows turn too, into d_q_out (not in place).  A position behind the table's
+ * end is dropped; so are K and V of one whose page is none of the pool's (a negative number, say). */
+typedef struct vnr_kv_append_desc {
+  int32_t batch, heads, rows;              /* heads: of d_q */
+  const int32_t *d_cu, *d_context, *d_table; int32_t table_width;      /* [batch + 1], [batch], [batch][table_width] */
+  const void *d_k, *d_v; int64_t ldk, ldv;
+  const void *d_q; void *d_q_out; int64_t ldq, ldqo;                   /* NULL, NULL: keys and values only */
+  const float *d_rotation; int32_t rotation_rows, rot_dim, interleaved;/* rotation_rows >= table_width * page_size */
+} vnr_kv_append_desc;
+int vnr_op_kv_append(vnr_handle h, const vnr_kv_cache *cache, const vnr_kv_append_desc *desc);
+/* Attention of the new rows over everything the cache holds of their sequence, themselves included (append first): row d_cu[b] + i sees
+ * positions 0 .. d_context[b] + i.  One new row a sequence is a decoding step; a whole chunk of a prompt works the same way.  max_new /
+ * max_context: the host's bounds for the new rows and for context + new rows of any sequence (positions from max_context on are not
+ * seen; max_new only chooses the launch).  A page number outside the pool reads as zeros. */
+typedef struct vnr_paged_attention_desc {
+  int32_t batch, heads, rows;
+  const int32_t *d_cu, *d_context, *d_table; int32_t table_width;
+  int32_t max_new, max_context;
+  float   scale;
+  const void *d_q; int64_t ldq;
+  void *d_out; int64_t ldo;
+  float *d_lse;                            /* [heads][rows] or NULL */
+} vnr_paged_attention_desc;
+int vnr_op_paged_attention(vnr_handle h, const vnr_kv_cache *cache, const vnr_paged_attention_desc *desc);
 
 /* ---- vocoder step after the path: reference audio/audio.py ---------------------------------
  * Audio.inv_mel_spectrogram up to the Griffin-Lim input (audio.py:81-84): _denormalize (:206-216) -> + ref_level_db ->

@@ -1,0 +1,583 @@
+"""Operators on packed sequences and on the paged cache (vaenar_tts_amd/sequence.py) against their definitions in 64 bits.
+
+Tolerances are element by element and come from the arithmetic (before any run), with u = half a step of the operands' type, h = 2^-24:
+  logits    e_s = (D + 4) h max_ij sum_d |q||k| scale          products and sums of D terms in 32 bits, the exponential's argument
+  out       u |out| + (u + 2 e_s + (n + 16) h) sum_j p|v|       the result's rounding, the probabilities' rounding, 32-bit sums of n terms
+  lse       e_s + (n + 16) h + 4 h |lse|
+  dS        u |dS| + (2 e_s + 32 h) |dS| + P (e_dP + e_delta), e_dP = (D + 4) h sum|dO||v|,
+            e_delta = sum_d |dO| e_out + (D + 4) h sum|dO||out|
+  gradients u |g| + scale (sum e_dS |x| + (n + 16) h sum |dS||x|), dV with P in the place of dS"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from vaenar_tts_amd import _lib, sequence
+from vaenar_tts_amd.configs import tiny_hps
+
+H24 = 2.0 ** -24
+KINDS = {"f32": (np.float32, 2.0 ** -24), "f16": (np.float16, 2.0 ** -11), "bf16": (np.uint16, 2.0 ** -8)}
+
+
+def store(x, kind):
+    return sequence.to_bf16(x) if kind == "bf16" else np.ascontiguousarray(x, KINDS[kind][0])
+
+
+def value(x):
+    return (sequence.from_bf16(x) if x.dtype == np.uint16 else x).astype(np.float64)
+
+
+def starts(lens, front=0):
+    return (np.concatenate([[0], np.cumsum(lens)]) + front).astype(np.int32)
+
+
+# ---- the definition -------------------------------------------------------------------------------------------------------------------
+def definition(q, k, v, cu_q, cu_k, causal, scale, u, dout=None, first=None):
+    """out, lse (and the gradients) in 64 bits with their element-wise tolerances: dict name -> (value, tolerance); rows outside the
+    sequences are NaN.  ``first``: keys in front of row 0 per sequence (a cache) instead of causal's nk - nq."""
+    H, G, D = q.shape[1], k.shape[1], q.shape[2]
+    new = lambda *s: [np.full(s, np.nan), np.full(s, np.nan)]
+    r = {"out": new(*q.shape), "lse": new(H, len(q))}
+    if dout is not None:
+        r.update(dq=new(*q.shape), dk=new(*k.shape), dv=new(*k.shape))
+    for b in range(len(cu_q) - 1):
+        iq, ik = slice(cu_q[b], cu_q[b + 1]), slice(cu_k[b], cu_k[b + 1])
+        nq, nk = cu_q[b + 1] - cu_q[b], cu_k[b + 1] - cu_k[b]
+        if dout is not None:
+            for n in ("dk", "dv"):
+                for x in r[n]:
+                    x[ik] = 0
+        for h in range(H):
+            g = h // (H // G)
+            Q, K, V = q[iq, h], k[ik, g], v[ik, g]
+            ahead = nk - nq if first is None else first[b]
+            see = np.arange(nk) <= np.arange(nq)[:, None] + ahead if causal else np.ones((nq, nk), bool)
+            x = np.where(see, Q @ K.T * scale, -np.inf) if nk else np.zeros((nq, 0))
+            e_s = (D + 4) * H24 * scale * (np.where(see, np.abs(Q) @ np.abs(K).T, 0).max(initial=0))
+            m = x.max(1, initial=-np.inf)[:, None]
+            m = np.where(np.isfinite(m), m, 0)
+            with np.errstate(divide="ignore"):
+                p = np.exp(x - m)
+                s = p.sum(1, keepdims=True)
+                p = np.where(s > 0, p / np.where(s > 0, s, 1), 0)
+                lse = (m + np.log(s))[:, 0]
+            sums = (nk + 16) * H24
+            out, A = p @ V, p @ np.abs(V)
+            e_out = u * np.abs(out) + (u + 2 * e_s + sums) * A
+            r["out"][0][iq, h], r["out"][1][iq, h] = out, e_out
+            r["lse"][0][h, iq], r["lse"][1][h, iq] = lse, e_s + sums + 4 * H24 * np.abs(np.where(np.isfinite(lse), lse, 0))
+            if dout is None:
+                continue
+            dO = dout[iq, h]
+            dP = dO @ V.T
+            delta = (dO * out).sum(1, keepdims=True)
+            dS = p * (dP - delta)
+            e_dP = (D + 4) * H24 * (np.abs(dO) @ np.abs(V).T)
+            e_delta = (np.abs(dO) * e_out).sum(1, keepdims=True) + (D + 4) * H24 * (np.abs(dO) * np.abs(out)).sum(1, keepdims=True)
+            e_dS = (u + 2 * e_s + 32 * H24) * np.abs(dS) + p * (e_dP + e_delta) * (1 + u)
+            e_p = (u + 2 * e_s + 32 * H24) * p
+            n_i = (nq * (H // G) + 16) * H24
+            dq = scale * dS @ K
+            r["dq"][0][iq, h] = dq
+            r["dq"][1][iq, h] = u * np.abs(dq) + scale * (e_dS @ np.abs(K) + sums * np.abs(dS) @ np.abs(K))
+            r["dk"][0][ik, g] += scale * dS.T @ Q
+            r["dk"][1][ik, g] += scale * (e_dS.T @ np.abs(Q) + n_i * np.abs(dS).T @ np.abs(Q))
+            r["dv"][0][ik, g] += p.T @ dO
+            r["dv"][1][ik, g] += e_p.T @ np.abs(dO) + n_i * p.T @ np.abs(dO)
+    if dout is not None:
+        for n in ("dk", "dv"):
+            r[n][1] += u * np.abs(r[n][0])
+    return r
+
+
+TINY = 2.0 ** -24          # the smallest step of float16: below its normal range a rounding is absolute
+
+
+def close(got, want, what, kind="f32"):
+    w, tol = want
+    live = ~np.isnan(w)
+    g = value(got)
+    inf = live & np.isinf(w)
+    assert (g[inf] == w[inf]).all(), what
+    fin = live & ~inf
+    off = np.abs(g[fin] - w[fin]) - (tol[fin] + (TINY if kind == "f16" else 1e-30))
+    assert off.size == 0 or off.max() <= 0, "%s: %g beyond its tolerance (worst value %g)" % (what, off.max(), np.abs(g[fin] - w[fin]).max())
+
+
+# ---- CPU ------------------------------------------------------------------------------------------------------------------------------
+def test_definition_gradients_match_differences():
+    """The gradients the tests hold the kernels to, against central differences of the definition's own output."""
+    r = np.random.default_rng(3)
+    cu_q, cu_k = starts([3, 4]), starts([5, 2])
+    q, k, v, w = r.standard_normal((7, 4, 8)), r.standard_normal((7, 2, 8)), r.standard_normal((7, 2, 8)), r.standard_normal((7, 4, 8))
+    f = lambda q, k, v: (definition(q, k, v, cu_q, cu_k, True, 0.4, 0)["out"][0] * w).sum()
+    d = definition(q, k, v, cu_q, cu_k, True, 0.4, 0, dout=w)
+    eps = 1e-6
+    for name, x in (("dq", q), ("dk", k), ("dv", v)):
+        for at in [(0, 0, 0), (2, 1, 3), (4, 0, 7), (6, 1, 5), (3, 0, 1)]:
+            hi, lo = x.copy(), x.copy()
+            hi[at] += eps
+            lo[at] -= eps
+            a = [{"dq": q, "dk": k, "dv": v}[n] for n in ("dq", "dk", "dv")]
+            i = ("dq", "dk", "dv").index(name)
+            num = (f(*(a[:i] + [hi] + a[i + 1:])) - f(*(a[:i] + [lo] + a[i + 1:]))) / (2 * eps)
+            assert abs(num - d[name][0][at]) < 1e-7, (name, at)
+
+
+def test_bfloat16_bits():
+    x = np.array([1, 1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8, -2.5, 0, 3e38, np.inf, -np.inf, 1e-40], np.float32)
+    y = sequence.from_bf16(sequence.to_bf16(x))
+    assert list(y[:5]) == [1, 1, 1 + 2.0 ** -6, -2.5, 0] and np.isinf(y[6]) and np.isinf(y[7])
+    assert np.isnan(sequence.from_bf16(sequence.to_bf16(np.float32([np.nan]))))[0]
+    assert np.abs(y[5] / x[5] - 1) <= 2.0 ** -8
+
+
+class Fake:
+    """An engine that only lends its name to arrays (nothing is launched: every call below is refused)."""
+    handle = None
+
+    def call(self, *a, **k):
+        raise AssertionError("a refused call reached the library")
+
+
+def fake(shape, dtype=np.float16):
+    return _lib.DeviceArray(Fake(), shape, dtype, ptr=0x1000, owner=None)
+
+
+def test_python_refusals():
+    e, q, k = Fake(), fake((6, 4, 64)), fake((6, 2, 64))
+    cu, lse = fake((3,), np.int32), fake((4, 6), np.float32)
+    ok = dict(out=q, lse=lse)
+    for bad in (dict(k=fake((5, 2, 32))), dict(v=fake((6, 1, 64))), dict(cu_q=fake((3,), np.float32)), dict(cu_k=fake((4,), np.int32)),
+                dict(q=fake((6, 4, 64), np.float64)), dict(k=fake((6, 2, 64), np.float32)), dict(lse=fake((6, 4), np.float32)),
+                dict(out=fake((6, 4, 32))), dict(q=fake((6, 256)))):
+        a = dict(q=q, k=k, v=k, cu_q=cu, **ok)
+        a.update(bad)
+        with pytest.raises(_lib.VnrError):
+            sequence.packed_attention(e, **a)
+    for bad in (dict(dout=fake((6, 4, 32))), dict(dk=fake((6, 4, 64))), dict(dq=fake((6, 4, 64), np.float32))):
+        a = dict(dout=q, q=q, k=k, v=k, out=q, lse=lse, cu_q=cu, dq=q, dk=k, dv=k)
+        a.update(bad)
+        with pytest.raises(_lib.VnrError):
+            sequence.packed_attention_grad(e, **a)
+    with pytest.raises(_lib.VnrError):
+        sequence.PagedCache(e, fake((4, 2, 16, 64)), fake((4, 2, 32, 64)))
+    with pytest.raises(_lib.VnrError):
+        sequence.PagedCache(e, fake((4, 2, 64)), fake((4, 2, 64)))
+    c = sequence.PagedCache(e, fake((4, 2, 16, 64)), fake((4, 2, 16, 64)))
+    ctx, table = fake((2,), np.int32), fake((2, 3), np.int32)
+    for bad in (dict(k=fake((6, 4, 64))), dict(v=fake((5, 2, 64))), dict(context=fake((3,), np.int32)), dict(table=fake((3, 3), np.int32)),
+                dict(q=fake((5, 4, 64))), dict(q_out=q), dict(rotation=fake((48, 64))), dict(k=fake((6, 2, 64), np.float32))):
+        a = dict(k=k, v=k, cu=cu, context=ctx, table=table)
+        a.update(bad)
+        with pytest.raises(_lib.VnrError):
+            c.append(**a)
+    for bad in (dict(q=fake((6, 4, 32))), dict(out=fake((6, 2, 64))), dict(lse=fake((6, 4), np.float32)), dict(q=fake((6, 4, 64), np.float32))):
+        a = dict(q=q, cu=cu, context=ctx, table=table, max_new=4, max_context=40, out=q)
+        a.update(bad)
+        with pytest.raises(_lib.VnrError):
+            c.attend(**a)
+
+
+def refused(name, *structs):
+    lib = _lib.load()
+    assert getattr(lib, name)(None, *[C.byref(s) for s in structs]) == -1
+    return lib.vnr_last_error(None).decode()
+
+
+def packed_desc(**kw):
+    d = dict(dtype=1, batch=2, heads=4, kv_heads=2, head_dim=64, causal=1, scale=0.125, rows_q=6, rows_k=6, d_cu_q=64, d_cu_k=64, d_q=4096, d_k=4096, d_v=4096,
+             ldq=256, ldk=128, ldv=128, d_out=4096, ldo=256, d_lse=None)
+    d.update(kw)
+    return _lib.vnr_packed_attention_desc(**d)
+
+
+def test_library_refusals_of_packed_calls():
+    """The library's own checks come before any use of the handle: they run here without a GPU, on pointers that nothing touches."""
+    for bad, word in ((dict(dtype=3), "dtype"), (dict(batch=0), "batch"), (dict(heads=3), "multiple of kv_heads"), (dict(kv_heads=0), "kv_heads"),
+                      (dict(head_dim=60), "head_dim"), (dict(head_dim=136), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(scale=0.0), "scale"),
+                      (dict(scale=float("nan")), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(rows_q=-1), "row count"),
+                      (dict(d_cu_q=None), "starts"), (dict(d_cu_k=None), "starts"), (dict(d_q=None), "q is null"), (dict(d_k=4104), "aligned"),
+                      (dict(ldq=248), "stride"), (dict(ldv=129), "stride"), (dict(ldk=64), "stride"), (dict(d_out=None), "out is null"), (dict(), "null handle")):
+        assert word in refused("vnr_op_packed_attention", packed_desc(**bad)), bad
+    g = dict(d_dout=4096, lddo=256, d_dq=4096, d_dk=4096, d_dv=4096, lddq=256, lddk=128, lddv=128)
+    for bad, word in ((dict(d_dout=None), "dout"), (dict(lddq=128), "dq"), (dict(d_dk=4100), "dk"), (dict(lddv=100), "dv"), (dict(), "null handle")):
+        assert word in refused("vnr_op_packed_attention_grad", packed_desc(d_lse=64), _lib.vnr_packed_attention_grad(**{**g, **bad})), bad
+    assert "lse" in refused("vnr_op_packed_attention_grad", packed_desc(), _lib.vnr_packed_attention_grad(**g))
+
+
+def test_library_refusals_of_cache_calls():
+    cache = dict(dtype=1, kv_heads=2, head_dim=64, pages=8, page_size=16, d_k=4096, d_v=4096)
+    app = dict(batch=2, heads=4, rows=6, d_cu=64, d_context=64, d_table=64, table_width=3, d_k=1 << 20, d_v=1 << 20, ldk=128, ldv=128, d_q=1 << 20, d_q_out=2 << 20,
+               ldq=256, ldqo=256, d_rotation=64, rotation_rows=48, rot_dim=64, interleaved=0)
+    att = dict(batch=2, heads=4, rows=6, d_cu=64, d_context=64, d_table=64, table_width=3, max_new=4, max_context=40, scale=0.125, d_q=4096, ldq=256, d_out=4096,
+               ldo=256, d_lse=None)
+    A, P, K = _lib.vnr_kv_append_desc, _lib.vnr_paged_attention_desc, _lib.vnr_kv_cache
+    for bad, word in ((dict(page_size=12), "page_size"), (dict(page_size=0), "page_size"), (dict(page_size=8192), "page_size"), (dict(pages=0), "pages"),
+                      (dict(d_k=None), "pools"), (dict(d_v=4104), "pools"), (dict(dtype=-1), "dtype"), (dict(head_dim=130), "head_dim")):
+        assert word in refused("vnr_op_kv_append", K(**{**cache, **bad}), A(**app)), bad
+        assert word in refused("vnr_op_paged_attention", K(**{**cache, **bad}), P(**att)), bad
+    for bad, word in ((dict(rows=-1), "row count"), (dict(d_k=None), "k is null"), (dict(ldv=120), "stride"), (dict(d_q_out=None), "together"),
+                      (dict(d_q=None), "together"), (dict(d_q_out=1 << 20), "overlaps"), (dict(d_q_out=(1 << 20) + 512), "overlaps"), (dict(rot_dim=72), "rot_dim"),
+                      (dict(rot_dim=24), "rot_dim"), (dict(rot_dim=20, interleaved=1), "rot_dim"), (dict(rot_dim=-16), "rot_dim"), (dict(d_rotation=None), "table is null"),
+                      (dict(rotation_rows=47), "cover"), (dict(table_width=0), "table_width"), (dict(table_width=1 << 28), "table_width"),
+                      (dict(d_cu=None), "starts"), (dict(heads=3), "heads"), (dict(), "null handle"),
+                      (dict(d_q=None, d_q_out=None), "null handle"),
+                      # q and q_out as two column blocks of one matrix do not overlap
+                      (dict(d_q_out=(1 << 20) + 512, ldq=512, ldqo=512), "null handle"), (dict(d_q_out=(1 << 20) + 256, ldq=512, ldqo=512), "overlaps")):
+        assert word in refused("vnr_op_kv_append", K(**cache), A(**{**app, **bad})), bad
+    for bad, word in ((dict(max_new=0), "max_new"), (dict(max_context=0), "max_context"), (dict(scale=0.0), "scale"), (dict(d_q=None), "q is null"), (dict(heads=5), "heads"),
+                      (dict(ldo=200), "stride"), (dict(d_table=None), "table"), (dict(), "null handle")):
+        assert word in refused("vnr_op_paged_attention", K(**cache), P(**{**att, **bad})), bad
+
+
+def test_sequence_structs_match_the_header_layout(tmp_path):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = ["vnr_packed_attention_desc", "vnr_packed_attention_grad", "vnr_kv_cache", "vnr_kv_append_desc", "vnr_paged_attention_desc"]
+    src = "#include <stdio.h>\n#include <stddef.h>\n#include \"vaenar_hip.h\"\nint main(void) {\n"
+    want = []
+    for n in names:
+        s = getattr(_lib, n)
+        src += 'printf("%%zu ", sizeof(%s));\n' % n
+        want.append(C.sizeof(s))
+        for f, _ in s._fields_:
+            src += 'printf("%%zu ", offsetof(%s, %s));\n' % (n, f)
+            want.append(getattr(s, f).offset)
+    open(tmp_path / "t.c", "w").write(src + "return 0; }\n")
+    subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(tmp_path / "t.c"), "-o", str(tmp_path / "t")])
+    assert [int(x) for x in subprocess.check_output([str(tmp_path / "t")]).split()] == want
+
+
+# ---- GPU ------------------------------------------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def eng():
+    e = _lib.Engine(tiny_hps(), 0)
+    yield e
+    e.close()
+
+
+def normal(r, kind, *shape):
+    return store(r.standard_normal(shape).astype(np.float32), kind)
+
+
+PACKED = [
+    # lens of queries, lens of keys (None: the same), heads, kv_heads, head_dim, causal
+    ([1], None, 1, 1, 64, True),
+    ([1, 2, 3, 0, 5], None, 4, 2, 64, True),
+    ([33, 64, 65], None, 4, 4, 64, False),
+    ([128, 129, 1, 127], None, 2, 1, 128, True),
+    ([200, 0, 77], None, 5, 1, 80, True),
+    ([31, 32, 100], None, 8, 2, 8, False),
+    ([130, 7], None, 3, 3, 104, True),
+    ([5, 40, 1, 3], [70, 40, 200, 0], 4, 2, 64, True),            # more keys than rows, and a sequence without keys
+    ([70, 150, 12], [5, 131, 12], 2, 1, 128, True),               # more rows than keys: the first rows see nothing
+    ([3, 260], [260, 3], 2, 2, 72, False),
+    ([0, 0, 9], [4, 0, 9], 2, 1, 64, True),                       # keys that no row sees
+    ([300], None, 1, 1, 128, True),
+]
+IDS = ["-".join([str(i)]) for i in range(len(PACKED))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", PACKED, ids=IDS)
+def test_packed_attention_and_gradient(eng, case, kind):
+    lq, lk, H, G, D, causal = case
+    u = KINDS[kind][1]
+    r = np.random.default_rng(sum(lq) * 7 + H + D)
+    cu_q = starts(lq, 2)
+    cu_k = cu_q if lk is None else starts(lk, 3)
+    nq, nk = cu_q[-1] + 3, cu_k[-1] + (3 if lk is None else 1)    # rows in front of the first sequence and behind the last
+    q, k, v, do = (normal(r, kind, n, h, D) for n, h in ((nq, H), (nk, G), (nk, G), (nq, H)))
+    bad = store(np.float32([np.nan]), kind)[0]
+    for x, cu in ((q, cu_q), (k, cu_k), (v, cu_k), (do, cu_q)):   # what is in those rows is nobody's business
+        x[:cu[0]] = bad
+        x[cu[-1]:] = bad
+    scale = 1.3 / np.sqrt(D)
+    want = definition(value(q), value(k), value(v), cu_q, cu_k, causal, np.float64(np.float32(scale)), u, dout=value(do))
+    d = [eng.to_device(x) for x in (q, k, v, do)]
+    cq = eng.to_device(cu_q)
+    ck = cq if lk is None else eng.to_device(cu_k)
+    mark = store(np.full(1, 7.0, np.float32), kind)[0]
+    filled = lambda x: eng.to_device(np.full(x.shape, mark, x.dtype))
+    out, dq, dk, dv = filled(q), filled(q), filled(k), filled(k)
+    lse = eng.to_device(np.full((H, nq), 7.0, np.float32))
+    sequence.packed_attention(eng, d[0], d[1], d[2], cq, None if lk is None else ck, causal, scale, out, lse)
+    sequence.packed_attention_grad(eng, d[3], d[0], d[1], d[2], out, lse, cq, None if lk is None else ck, causal, scale, dq, dk, dv)
+    for name, a in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        got = a.numpy()
+        close(got, want[name], name, kind)
+        cu = cu_k if name in ("dk", "dv") else cu_q
+        assert (got[:cu[0]] == mark).all() and (got[cu[-1]:] == mark).all(), name + ": rows outside the sequences were written"
+    got = lse.numpy()
+    close(got, want["lse"], "lse")
+    assert (got[:, :cu_q[0]] == 7).all() and (got[:, cu_q[-1]:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_packed_attention_on_column_blocks(eng, kind):
+    """q, k, v, dout as column blocks of one projection's rows, results as column blocks too: the rest of the rows stays."""
+    H, G, D, u = 4, 2, 64, KINDS[kind][1]
+    lens = [40, 3, 90]
+    cu = starts(lens)
+    n, width = cu[-1], (H + 2 * G) * D + 8
+    r = np.random.default_rng(9)
+    x, do = normal(r, kind, n, width), normal(r, kind, n, H * D + 16)
+    cut = lambda a, o, h: value(a[:, o:o + h * D]).reshape(n, h, D)
+    q, k, v = cut(x, 0, H), cut(x, H * D, G), cut(x, (H + G) * D, G)
+    want = definition(q, k, v, cu, cu, True, D ** -0.5, u, dout=cut(do, 16, H))
+    dx, ddo, c = eng.to_device(x), eng.to_device(do), eng.to_device(cu)
+    g = eng.to_device(x)                                          # gradients into the same columns of a matrix like it
+    o = eng.to_device(np.zeros((n, H * D + 24), x.dtype))
+    a = [dx.view(0, (n, H, D)), dx.view(H * D, (n, G, D)), dx.view((H + G) * D, (n, G, D))]
+    ov, lse = o.view(8, (n, H, D)), eng.empty((H, n))
+    ld = dict(ldq=width, ldk=width, ldv=width, ldo=H * D + 24)
+    sequence.packed_attention(eng, *a, c, out=ov, lse=lse, **ld)
+    sequence.packed_attention_grad(eng, ddo.view(16, (n, H, D)), *a, ov, lse, c, dq=g.view(0, (n, H, D)), dk=g.view(H * D, (n, G, D)),
+                                   dv=g.view((H + G) * D, (n, G, D)), lddout=H * D + 16, lddq=width, lddk=width, lddv=width, **ld)
+    oh, gh = o.numpy(), g.numpy()
+    shaped = lambda a, o, h: a[:, o:o + h * D].reshape(n, h, D)
+    close(shaped(oh, 8, H), want["out"], "out", kind)
+    assert (oh[:, :8] == 0).all() and (oh[:, 8 + H * D:] == 0).all() and (gh[:, -8:] == x[:, -8:]).all()
+    for name, at, h in (("dq", 0, H), ("dk", H * D, G), ("dv", (H + G) * D, G)):
+        close(shaped(gh, at, h), want[name], name, kind)
+
+
+@pytest.mark.gpu
+def test_packed_gradient_has_the_same_bits_every_time(eng):
+    r = np.random.default_rng(4)
+    cu = starts([200, 90, 333])
+    q, k, v, do = (eng.to_device(normal(r, "bf16", cu[-1], h, 128)) for h in (8, 2, 2, 8))
+    c = eng.to_device(cu)
+    out, lse = sequence.packed_attention(eng, q, k, v, c)
+    a = [x.numpy() for x in sequence.packed_attention_grad(eng, do, q, k, v, out, lse, c)]
+    for _ in range(3):
+        assert all((x.numpy() == y).all() for x, y in zip(sequence.packed_attention_grad(eng, do, q, k, v, out, lse, c), a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_packed_attention_with_broken_starts(eng, kind):
+    """Starts that run backwards or leave the tensor: those sequences are empty or cut, the others are right, nothing else is written."""
+    H, D = 2, 64
+    r = np.random.default_rng(5)
+    q, k, v = (normal(r, kind, 50, H, D) for _ in range(3))
+    cu = np.int32([0, 20, 10, 1000])                              # 0..20; 20..10 is empty; 10..1000 is cut to 10..50
+    d, c = [eng.to_device(x) for x in (q, k, v)], eng.to_device(cu)
+    out, lse = sequence.packed_attention(eng, *d, c)
+    got = out.numpy()
+    assert np.isfinite(value(got)).all()
+    want = definition(value(q), value(k), value(v), starts([20]), starts([20]), True, D ** -0.5, KINDS[kind][1])
+    close(got[:10], [x[:10] for x in want["out"]], "out", kind)
+
+
+# ---- the cache ------------------------------------------------------------------------------------------------------------------------
+def turned(x, pos, rot, base, interleaved):
+    """[n, heads, D] turned by its positions, in 64 bits from the table's 32-bit entries"""
+    half = rot // 2
+    ang = np.asarray(pos, np.float64)[:, None] * base ** (-2.0 * np.arange(half) / rot)
+    cs, sn = (f(ang).astype(np.float32).astype(np.float64)[:, None] for f in (np.cos, np.sin))
+    y = x.copy()
+    i, j = (np.arange(0, rot, 2), np.arange(1, rot, 2)) if interleaved else (np.arange(half), np.arange(half, rot))
+    y[..., i], y[..., j] = x[..., i] * cs - x[..., j] * sn, x[..., j] * cs + x[..., i] * sn
+    return y
+
+
+def layout(r, totals, P, spare=2):
+    """A page table of shuffled pages for sequences of `totals` positions, and the pool's size"""
+    held = [-(-t // P) for t in totals]
+    pages = sum(held) + spare
+    order = r.permutation(pages).astype(np.int32)
+    table = np.full((len(totals), max(max(held), 1)), -1, np.int32)
+    at = 0
+    for b, n in enumerate(held):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return table, pages
+
+
+APPEND = [
+    # new, context, page, heads, kv_heads, head_dim, rot_dim, interleaved
+    ([1], [0], 16, 1, 1, 64, 64, False),
+    ([1, 1, 1], [5, 15, 16], 16, 8, 2, 128, 128, False),
+    ([7, 0, 33], [3, 9, 60], 8, 4, 4, 64, 32, False),
+    ([20, 5], [0, 100], 1, 3, 1, 80, 48, True),
+    ([40], [1000], 64, 5, 5, 8, 8, True),
+    ([3, 70], [2, 4000], 128, 4, 2, 104, 16, False),
+    ([3, 2], [2, 1], 16, 2, 2, 64, 0, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", APPEND, ids=[str(i) for i in range(len(APPEND))])
+def test_append(eng, case, kind):
+    new, ctx, P, H, G, D, rot, inter = case
+    u = KINDS[kind][1]
+    r = np.random.default_rng(sum(new) + P)
+    table, pages = layout(r, [n + c for n, c in zip(new, ctx)], P)
+    cu = starts(new, 1)
+    n = cu[-1] + 2
+    k, v, q = normal(r, kind, n, G, D), normal(r, kind, n, G, D), normal(r, kind, n, H, D)
+    kc, vc = normal(r, kind, pages, G, P, D), normal(r, kind, pages, G, P, D)
+    base = 500.0
+    dk, dv = eng.to_device(kc), eng.to_device(vc)
+    cache = sequence.PagedCache(eng, dk, dv)
+    table_rot = sequence.rotation_table(eng, table.shape[1] * P, rot, base) if rot else None
+    mark = store(np.full(1, 7.0, np.float32), kind)[0]
+    qo = eng.to_device(np.full(q.shape, mark, q.dtype))
+    cache.append(eng.to_device(k), eng.to_device(v), eng.to_device(cu), eng.to_device(np.int32(ctx)), eng.to_device(table), rotation=table_rot,
+                 q=eng.to_device(q), q_out=qo, interleaved=inter)
+    want_k, want_v, want_q = value(kc), vc.copy(), np.full(q.shape, np.nan)
+    touched = np.zeros(kc.shape, bool)
+    for b, m in enumerate(new):
+        pos = ctx[b] + np.arange(m)
+        kt, qt = value(k[cu[b]:cu[b + 1]]), value(q[cu[b]:cu[b + 1]])
+        if rot:
+            kt, qt = turned(kt, pos, rot, base, inter), turned(qt, pos, rot, base, inter)
+        want_q[cu[b]:cu[b + 1]] = qt
+        for i, p in enumerate(pos):
+            page = table[b, p // P]
+            want_k[page, :, p % P], want_v[page, :, p % P] = kt[i], v[cu[b] + i]
+            touched[page, :, p % P] = True
+    # two products and a sum in 32 bits, one rounding; the table's own rounding of cos / sin is in the reference (h: it may differ by one)
+    tol = lambda w: (u + 4 * H24) * np.abs(w) + 12 * H24
+    gk, gq = dk.numpy(), qo.numpy()
+    assert (dv.numpy() == want_v).all()
+    assert (gk[~touched] == kc[~touched]).all()
+    close(gk, (want_k, tol(want_k)), "k", kind)
+    close(gq, (want_q, np.where(np.isnan(want_q), 0, tol(want_q))), "q", kind)
+    assert (gq[0] == mark).all() and (gq[cu[-1]:] == mark).all()
+
+
+@pytest.mark.gpu
+def test_rotation_table_of_far_positions(eng):
+    t = sequence.rotation_table(eng, 100003, 64, 10000.0).numpy()
+    for p in (0, 1, 4097, 65537, 100002):
+        ang = p * 10000.0 ** (-2.0 * np.arange(32) / 64)
+        assert np.abs(t[p] - np.concatenate([np.cos(ang), np.sin(ang)])).max() <= 2 * H24
+    assert t.shape == (100003, 64)
+
+
+@pytest.mark.gpu
+def test_append_drops_what_has_no_place(eng):
+    """Pages outside the pool, positions behind the table: nothing is written for them, the rest is; the queries turn where they have an angle."""
+    r = np.random.default_rng(8)
+    P, G, D, pages = 4, 2, 64, 5
+    k, v = normal(r, "f16", 12, G, D), normal(r, "f16", 12, G, D)
+    kc = normal(r, "f16", pages, G, P, D)
+    table = np.int32([[3, -1], [1 << 30, 0], [2, 5]])
+    cu, ctx = starts([6, 4, 2]), np.int32([0, 6, 3])             # 0: positions 0..5 (page -1 from 4); 1: 6..9 (8, 9 behind the table); 2: 3, 4 (page 5)
+    dk, dv = eng.to_device(kc), eng.to_device(kc)
+    sequence.PagedCache(eng, dk, dv).append(eng.to_device(k), eng.to_device(v), eng.to_device(cu), eng.to_device(ctx), eng.to_device(table))
+    want = kc.copy()
+    for row, page, slot in ((0, 3, 0), (1, 3, 1), (2, 3, 2), (3, 3, 3), (6, 0, 2), (7, 0, 3), (10, 2, 3)):
+        want[page, :, slot] = k[row]
+    assert (dk.numpy() == want).all()
+
+
+PAGED = [
+    # new, context, page, heads, kv_heads, head_dim
+    ([1], [0], 16, 1, 1, 64),
+    ([1, 1, 0, 1], [1, 63, 7, 64], 16, 4, 4, 64),
+    ([1, 1], [1000, 3], 16, 8, 2, 128),
+    ([1, 1, 1], [127, 2049, 700], 1, 5, 1, 80),
+    ([5, 2, 1], [300, 0, 33], 32, 8, 2, 64),
+    ([40, 3], [100, 513], 64, 4, 1, 128),
+    ([130, 0, 65], [5, 60, 0], 8, 3, 3, 96),
+    ([9, 200], [1500, 1], 128, 4, 2, 64),
+    ([1], [5000], 4096, 2, 1, 8),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", PAGED, ids=[str(i) for i in range(len(PAGED))])
+def test_paged_attention(eng, case, kind):
+    new, ctx, P, H, G, D = case
+    u = KINDS[kind][1]
+    r = np.random.default_rng(sum(new) + sum(ctx))
+    totals = [n + c for n, c in zip(new, ctx)]
+    table, pages = layout(r, totals, P)
+    # a pool whose unused places hold NaN: behind a sequence's last position, and in pages that are nobody's
+    bad = store(np.float32([np.nan]), kind)[0]
+    kc, vc = np.full((pages, G, P, D), bad, KINDS[kind][0]), np.full((pages, G, P, D), bad, KINDS[kind][0])
+    k, v = normal(r, kind, sum(totals), G, D), normal(r, kind, sum(totals), G, D)
+    at = starts(totals)
+    for b, n in enumerate(totals):
+        for p in range(n):
+            kc[table[b, p // P], :, p % P], vc[table[b, p // P], :, p % P] = k[at[b] + p], v[at[b] + p]
+    cu = starts(new, 1)
+    n = cu[-1] + 2
+    q = normal(r, kind, n, H, D)
+    q[0], q[cu[-1]:] = bad, bad
+    want = definition(value(q), value(k), value(v), cu, at, True, D ** -0.5, u, first=ctx)
+    mark = store(np.full(1, 7.0, np.float32), kind)[0]
+    out, lse = eng.to_device(np.full(q.shape, mark, q.dtype)), eng.to_device(np.full((H, n), 7.0, np.float32))
+    cache = sequence.PagedCache(eng, eng.to_device(kc), eng.to_device(vc))
+    cache.attend(eng.to_device(q), eng.to_device(cu), eng.to_device(np.int32(ctx)), eng.to_device(table), max(max(new), 1), max(totals), out=out, lse=lse)
+    got, gl = out.numpy(), lse.numpy()
+    close(got, want["out"], "out", kind)
+    close(gl, want["lse"], "lse")
+    assert (got[0] == mark).all() and (got[cu[-1]:] == mark).all() and (gl[:, 0] == 7).all() and (gl[:, cu[-1]:] == 7).all()
+    # bounds that are wider than the batch: another launch, the same values
+    wide = eng.to_device(np.full(q.shape, mark, q.dtype))
+    cache.attend(eng.to_device(q), eng.to_device(cu), eng.to_device(np.int32(ctx)), eng.to_device(table), 10000, 1 << 20, out=wide)
+    close(wide.numpy(), want["out"], "out (wide bounds)", kind)
+
+
+@pytest.mark.gpu
+def test_paged_attention_reads_absent_pages_as_zeros(eng):
+    r = np.random.default_rng(2)
+    P, G, D = 16, 1, 64
+    kc, vc = normal(r, "f32", 3, G, P, D), normal(r, "f32", 3, G, P, D)
+    q = normal(r, "f32", 2, 2, D)
+    table = np.int32([[1, -5, 2], [7, 0, 1 << 30]])
+    cu, ctx = starts([1, 1]), np.int32([40, 47])
+    full = np.zeros((2, 48, G, D)), np.zeros((2, 48, G, D))
+    for b in range(2):
+        for j in range(3):
+            if 0 <= table[b, j] < 3:
+                full[0][b, 16 * j:16 * j + 16], full[1][b, 16 * j:16 * j + 16] = (x[table[b, j]].transpose(1, 0, 2) for x in (kc, vc))
+    out = sequence.PagedCache(eng, eng.to_device(kc), eng.to_device(vc)).attend(eng.to_device(q), eng.to_device(cu), eng.to_device(ctx), eng.to_device(table), 1, 48)
+    want = definition(value(q), full[0].reshape(96, G, D), full[1].reshape(96, G, D), cu, starts([48, 48]), True, D ** -0.5, 2.0 ** -24, first=[40, 47])
+    close(out.numpy(), want["out"], "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_prompt_then_chunks_then_single_rows(eng, kind):
+    """The operators as they are used together: prompts through packed attention and append, a chunk, then one row at a time -- every row's
+    output has to be what attention over the whole sequence gives."""
+    H, G, D, P, u = 4, 2, 64, 16, KINDS[kind][1]
+    r = np.random.default_rng(11)
+    steps = [[37, 5], [20, 64], [1, 1], [1, 1], [0, 1]]
+    total = [sum(s[b] for s in steps) for b in range(2)]
+    table, pages = layout(r, total, P)
+    cache = sequence.PagedCache.empty(eng, pages, G, P, D, KINDS[kind][0])
+    rot, dt = sequence.rotation_table(eng, table.shape[1] * P, D), eng.to_device(table)
+    kept = {n: [[], []] for n in ("q", "k", "v", "out")}
+    ctx = [0, 0]
+    for i, new in enumerate(steps):
+        n = sum(new)
+        q, k, v = normal(r, kind, n, H, D), normal(r, kind, n, G, D), normal(r, kind, n, G, D)
+        dq, dk, dv, cu, c = (eng.to_device(x) for x in (q, k, v, starts(new), np.int32(ctx)))
+        qt = cache.append(dk, dv, cu, c, dt, rotation=rot, q=dq)
+        kt = eng.empty((n, G, D), KINDS[kind][0])                 # the rotated keys, through the query side of another append
+        cache.append(dk, dv, cu, c, dt, rotation=rot, q=dk, q_out=kt)
+        if i == 0:
+            out, _ = sequence.packed_attention(eng, qt, kt, dv, cu)
+        else:
+            out = cache.attend(qt, cu, c, dt, max(new), max(x + y for x, y in zip(ctx, new)))
+        got, turned_q, turned_k, s = out.numpy(), qt.numpy(), kt.numpy(), starts(new)
+        for b in range(2):
+            for name, x in (("q", turned_q), ("k", turned_k), ("v", v), ("out", got)):
+                kept[name][b].append(x[s[b]:s[b + 1]])
+            ctx[b] += new[b]
+    cu = starts(total)
+    whole = {n: np.concatenate([np.concatenate(kept[n][b]) for b in range(2)]) for n in kept}
+    want = definition(value(whole["q"]), value(whole["k"]), value(whole["v"]), cu, cu, True, D ** -0.5, u)
+    close(whole["out"], want["out"], "out", kind)

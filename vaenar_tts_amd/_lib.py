@@ -11,7 +11,7 @@ import numpy as np
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libvaenar_hip.so")
-ABI_VERSION = 6
+ABI_VERSION = 7
 VNR_ERR_RANGE = -6
 
 ACT = {"identity": 0, None: 0, "relu": 1, "tanh": 2}
@@ -65,6 +65,48 @@ class vnr_dense_desc(C.Structure):
     ]
 
 
+class vnr_packed_attention_desc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("causal", C.c_int32), ("scale", C.c_float), ("rows_q", C.c_int32), ("rows_k", C.c_int32),
+        ("d_cu_q", C.c_void_p), ("d_cu_k", C.c_void_p), ("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p),
+        ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("d_out", C.c_void_p), ("ldo", C.c_int64), ("d_lse", C.c_void_p),
+    ]
+
+
+class vnr_packed_attention_grad(C.Structure):
+    _fields_ = [
+        ("d_dout", C.c_void_p), ("lddo", C.c_int64), ("d_dq", C.c_void_p), ("d_dk", C.c_void_p), ("d_dv", C.c_void_p),
+        ("lddq", C.c_int64), ("lddk", C.c_int64), ("lddv", C.c_int64),
+    ]
+
+
+class vnr_kv_cache(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32),
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p),
+    ]
+
+
+class vnr_kv_append_desc(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("heads", C.c_int32), ("rows", C.c_int32),
+        ("d_cu", C.c_void_p), ("d_context", C.c_void_p), ("d_table", C.c_void_p), ("table_width", C.c_int32),
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("ldk", C.c_int64), ("ldv", C.c_int64),
+        ("d_q", C.c_void_p), ("d_q_out", C.c_void_p), ("ldq", C.c_int64), ("ldqo", C.c_int64),
+        ("d_rotation", C.c_void_p), ("rotation_rows", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32),
+    ]
+
+
+class vnr_paged_attention_desc(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("heads", C.c_int32), ("rows", C.c_int32),
+        ("d_cu", C.c_void_p), ("d_context", C.c_void_p), ("d_table", C.c_void_p), ("table_width", C.c_int32),
+        ("max_new", C.c_int32), ("max_context", C.c_int32), ("scale", C.c_float),
+        ("d_q", C.c_void_p), ("ldq", C.c_int64), ("d_out", C.c_void_p), ("ldo", C.c_int64), ("d_lse", C.c_void_p),
+    ]
+
+
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 _pd, _pi64 = C.POINTER(C.c_double), C.POINTER(C.c_int64)
 
@@ -102,6 +144,11 @@ PROTOTYPES = {
     "vnr_op_layer_norm": [_vp, _vp, _vp, _vp, _i, _i, _vp],
     "vnr_op_kernel_grad": [_vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "vnr_op_positional_encoding": [_vp, _i, _i, _f, _vp],
+    "vnr_op_packed_attention": [_vp, C.POINTER(vnr_packed_attention_desc)],
+    "vnr_op_packed_attention_grad": [_vp, C.POINTER(vnr_packed_attention_desc), C.POINTER(vnr_packed_attention_grad)],
+    "vnr_op_rotation_table": [_vp, _i, _i, C.c_double, _vp],
+    "vnr_op_kv_append": [_vp, C.POINTER(vnr_kv_cache), C.POINTER(vnr_kv_append_desc)],
+    "vnr_op_paged_attention": [_vp, C.POINTER(vnr_kv_cache), C.POINTER(vnr_paged_attention_desc)],
     "vnr_random_normal": [_vp, C.c_uint64, C.c_uint64, _f, _vp, _sz],
     "vnr_voc_mel_to_linear": [_vp, _vp, _vp, _i, _i, _i, _i, _f, _f, _f, _i, _f, _vp],
     "vnr_voc_griffin_lim": [_vp, _vp, _vp, C.c_uint64, _vp, _i, _i, _i, _i, _i, _i, _vp],

@@ -2,6 +2,7 @@
 // stream, and the extern "C" ABI declared in include/vaenar_hip.h.
 #include "../../include/vaenar_hip.h"
 #include "common.h"
+#include "sequence.h"
 #include <chrono>
 
 #include <dlfcn.h>
@@ -71,9 +72,9 @@ struct ProfRec { int cls; hipEvent_t e0, e1; double flops, bytes; };
 // "chain_ali": chain launches whose fused cross-attention also writes the alignments (the decoder's blocks since round 4)
 // training step only: "gemm_tn" kernel-gradient GEMMs (split), "bwd_chain" backward row-panel chains (split), "attn_bwd" attention backward (split)
 enum { CLS_GEMM = 0, CLS_ATTN_SELF, CLS_ATTN_CROSS, CLS_ATTN_CROSS_ALI, CLS_LN, CLS_MISC, CLS_GEMM_F32, CLS_CHAIN, CLS_CHAIN_ALI, CLS_GEMM_TN, CLS_BWD_CHAIN,
-       CLS_ATTN_BWD, CLS_COUNT };
+       CLS_ATTN_BWD, CLS_SEQ, CLS_COUNT };
 const char* kClsNames[CLS_COUNT] = {"gemm", "attn_self", "attn_cross", "attn_cross_ali", "layer_norm", "misc", "gemm_fp32", "chain", "chain_ali", "gemm_tn",
-                                    "bwd_chain", "attn_bwd"};
+                                    "bwd_chain", "attn_bwd", "sequence"};
 
 // Dropout sites (one mask stream per tf.keras.layers.Dropout instance of the path): encoder.py:70,87; utils.py:73,84
 // (prenet / postnet convolutions); utils.py:11-17 (posterior PreNet, two uses of one layer); posterior.py:99,122
@@ -208,6 +209,9 @@ struct vnr_context {
   // positional-encoding tables, keyed by (T, dim, step bits)
   std::map<std::tuple<int, int, uint32_t>, float*> pe_cache;
   std::map<int, float*> voc_tables;     // win_length -> [twiddles 2048 floats | Hann window win floats] (vocoder.hip)
+
+  void* seq_zero = nullptr;      // 64 bytes of zeros (sequence.inc)
+  int compute_units = 256;
 
   // instrumentation
   bool profiling = false;
@@ -1735,6 +1739,7 @@ int vnr_create(const vnr_config* cfg, int device, vnr_handle* out) {
   vnr_handle h = new vnr_context();
   h->cfg = *cfg;
   h->device = device;
+  { int cus = 0; if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess && cus > 0) h->compute_units = cus; }
   if (const char* e = getenv("VNR_CHAIN_ROWS64")) h->chain_rows64 = atoi(e) != 0;
   if (const char* e = getenv("VNR_CHAIN_WAVES4")) h->chain_waves4 = atoi(e) != 0;
   if (const char* e = getenv("VNR_CHAIN_SEGMENTS")) h->chain_segments = atoi(e) != 0;
@@ -1782,6 +1787,7 @@ int vnr_destroy(vnr_handle h) {
   if (h->range_flag) hipHostFree(h->range_flag);
   if (h->d_step_flag) hipFree(h->d_step_flag);
   if (h->amax_words) hipFree(h->amax_words);
+  if (h->seq_zero) hipFree(h->seq_zero);
   if (h->kv_stream) { hipStreamSynchronize(h->kv_stream); hipStreamDestroy(h->kv_stream); }
   if (h->kv_fork) hipEventDestroy(h->kv_fork);
   if (h->kv_done) hipEventDestroy(h->kv_done);
@@ -2682,6 +2688,8 @@ int vnr_op_kernel_grad(vnr_handle h, const float* d_x, int ldx, const float* d_d
   HIP_TRY(h, e);
   return VNR_OK;
 }
+
+#include "sequence.inc"
 
 // tf.random.normal(shape, stddev) on the device (prior.py:35, posterior.py:35)
 int vnr_random_normal(vnr_handle h, uint64_t seed, uint64_t offset, float stddev, float* d_out, size_t n) {
