@@ -21,10 +21,10 @@ struct SeqArgs {
   // a sequence's keys cut into `splits` pieces of `chunk` keys, joined by seq_join_kernel; part [splits][rows_q * heads][dim], ml [splits][rows_q * heads][2]
   int splits = 1, chunk = 0;
   float* part = nullptr; float* ml = nullptr;
-  const void* zero = nullptr;                                        // 16 bytes of zeros: where the loads of absent rows point
+  const void* zero = nullptr;                                        // 64 bytes of zeros: where the loads of absent rows point
 };
-// the launch that seq_plan() chose for these sizes: rows per workgroup, whether the waves share the keys (false: each takes keys of its own)
-struct SeqPlan { int shared = 1, rows = 128, splits = 1, chunk = 0; };
+// the launch that seq_plan() chose for these sizes: how many of a workgroup's four waves stand side by side along the rows (the others: along the keys)
+struct SeqPlan { int row_waves = 4, splits = 1, chunk = 0; };
 SeqPlan seq_plan(const SeqArgs& a, int compute_units);
 hipError_t launch_seq_fwd(const SeqArgs& a, const SeqPlan& p, hipStream_t s);
 hipError_t launch_seq_join(const SeqArgs& a, hipStream_t s);
@@ -35,7 +35,7 @@ struct SeqGradArgs {
   void *dq = nullptr, *dk = nullptr, *dv = nullptr; long long lddq = 0, lddk = 0, lddv = 0;
   float* delta = nullptr;                                            // [heads][rows_q] scratch: sum_d dout * out of every row
 };
-hipError_t launch_seq_grad(const SeqGradArgs& a, hipStream_t s);
+hipError_t launch_seq_grad(const SeqGradArgs& a, int compute_units, hipStream_t s);
 
 struct SeqAppendArgs {
   int dtype = 0, batch = 0, heads = 0, kv_heads = 0, dim = 0, rows = 0;
@@ -69,13 +69,18 @@ __device__ __forceinline__ f32x16 seq_mma(sq_f8 a, sq_f8 b, f32x16 c) {
   return c;
 }
 
-// Tiles in LDS: rows of DP elements, 16-byte chunks; chunk c of row r lies at c ^ (r & 7), so that the 32 rows that one matrix operand reads
-// at the same chunk spread over the banks (a row is 128, 256 or 512 bytes: without it they share eight lanes' worth of banks).
+// Tiles in LDS: rows of DP elements in 16-byte chunks; chunk c of row r lies at c ^ turn(r).  Two kinds of reads have to spread over the 64
+// banks (256 bytes): sixteen rows at one chunk (the phases of a 16-byte read take rows 0-3, 12-15, 20-27 together), and four consecutive rows
+// at four neighbouring chunks (half a wave of the transposing read).  With turn(r) = r % 8 the second kind met 4-fold conflicts: 62 % of the
+// LDS cycles of the backward kernels.
 template <typename T, int DP> struct SeqTile {
   static constexpr int kRow = DP * (int)sizeof(T);           // bytes
   static constexpr int kChunks = kRow / 16;
   static constexpr int kPer = 16 / (int)sizeof(T);           // elements of a chunk
-  static __device__ __forceinline__ int at(int r, int c) { return r * kRow + ((c ^ (r & 7)) << 4); }
+  static __device__ __forceinline__ int turn(int r) {        // rows of 128 bytes: two of them share the banks
+    return kChunks == 8 ? ((r & 2) << 1) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+  static __device__ __forceinline__ int at(int r, int c) { return r * kRow + ((c ^ turn(r)) << 4); }
 };
 // operand with rows along the lanes: elements 8 u .. 8 u + 7 of row r
 template <typename T, int DP>
@@ -119,16 +124,24 @@ template <typename T> __device__ __forceinline__ typename SeqVec<T>::v8 seq_pack
   for (int e = 0; e < 8; ++e) v[e] = x[8 * t + e];
   if constexpr (sizeof(T) == 4) return v; else return __builtin_convertvector(v, typename SeqVec<T>::v8);
 }
-// sixteen bytes (or thirty-two in 32 bits) of a row in memory: elements 8 u .. 8 u + 7, zeros where `ok` is false
-template <typename T> __device__ __forceinline__ typename SeqVec<T>::v8 seq_load8(const T* p, bool ok) {
-  typename SeqVec<T>::v8 v = {};
-  if (ok) v = *reinterpret_cast<const typename SeqVec<T>::v8*>(p);
-  return v;
+// elements 8 u .. 8 u + 7 of a row in memory, zeros where `ok` is false (read from `zero`: no branch)
+template <typename T> __device__ __forceinline__ typename SeqVec<T>::v8 seq_load8(const T* p, bool ok, const void* zero) {
+  return *reinterpret_cast<const typename SeqVec<T>::v8*>(ok ? (const void*)p : zero);
 }
 template <typename T> __device__ __forceinline__ void seq_store4(T* p, float a, float b, float c, float d) {
   const sq_f4 v = {a, b, c, d};
   if constexpr (sizeof(T) == 4) *reinterpret_cast<sq_f4*>(p) = v;
   else *reinterpret_cast<typename SeqVec<T>::v4*>(p) = __builtin_convertvector(v, typename SeqVec<T>::v4);
+}
+// operands that a loop keeps reading are waited for here, not by a counter wait that the compiler would repeat in every turn of the loop (and
+// that would drain the transfers on their way)
+template <typename V, int N> __device__ __forceinline__ void seq_settle(V (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const sq_f4* p = reinterpret_cast<const sq_f4*>(&x[i]);
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(V) / 16); ++j) asm volatile("" ::"v"(p[j]));
+  }
 }
 // the value of the lane itself and of the one 32 away, in either order
 __device__ __forceinline__ sq_f2 seq_pair(float x) {
@@ -139,42 +152,92 @@ __device__ __forceinline__ sq_f2 seq_pair(float x) {
 }
 __device__ __forceinline__ float seq_pair_max(float x) { const sq_f2 v = seq_pair(x); return fmaxf(v[0], v[1]); }
 __device__ __forceinline__ float seq_pair_sum(float x) { const sq_f2 v = seq_pair(x); return v[0] + v[1]; }
-// 16 bytes from memory straight to LDS: lane i's sixteen bytes land at dst + 16 i
-__device__ __forceinline__ void seq_dma16(const void* src, char* dst) {
-  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// 16 (4) bytes a lane from memory straight to LDS: lane i's land at dst + 16 i (4 i); dst is the same for the wave.  The compiler is not told
+// of the transfer -- it would drain all of them in front of every transposing read of LDS --: seq_dma_wait in front of the barrier behind
+// which the tile is read is the kernels' own duty.  (No register is written, and the counter waits that the compiler places for its own loads
+// only become longer by transfers it does not know.  m0, the transfer's destination, is set and used inside the block; nothing else in these
+// kernels uses it.)
+__device__ __forceinline__ unsigned seq_lds(const char* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p; }
+__device__ __forceinline__ void seq_dma16(const void* src, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+// the same from a scalar base and a 32-bit offset a lane: no address arithmetic in vector registers
+__device__ __forceinline__ void seq_dma16(const void* base, unsigned offset, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void seq_dma4(const void* src, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+// all but the newest `left` transfers have landed (a transfer lands in the order of its issue)
+template <int left = 0> __device__ __forceinline__ void seq_dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(left) : "memory"); }
+// every LDS read of the wave has been answered: what it read from may be overwritten
+__device__ __forceinline__ void seq_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The offsets of a wave's lanes in a transfer of 64 chunks (kRowsOf rows, `ld` bytes apart): they repeat every kPeriod transfers
+template <typename T, int DP> struct SeqLanes {
+  typedef SeqTile<T, DP> L;
+  static constexpr int kRowsOf = 64 / L::kChunks, kPeriod = 16 / kRowsOf;
+  unsigned at[kPeriod];
+  __device__ __forceinline__ void set(unsigned ld, int lane, int first) {         // first: the wave's first transfer of a tile
+#pragma unroll
+    for (int i = 0; i < kPeriod; ++i) {
+      const int r = lane / L::kChunks;
+      at[i] = r * ld + (((lane % L::kChunks) ^ L::turn((first + i) * kRowsOf + r)) << 4);
+    }
+  }
+};
+// a load through the scalar cache: `p` is the same for the wave and nobody writes there during the kernel
+__device__ __forceinline__ int seq_scalar(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int*)(unsigned long long)p;
 }
 
 // The sequence and the tile in it that a workgroup's tile index names: every sequence of n rows has ceil(n * mult / rows) tiles.  Starts that
-// run backwards or leave the tensor are clamped: such a sequence is empty, nothing outside the tensor is touched.
-struct SeqWhere { int b, tile, start, n; };
-__device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total, int mult, int rows, int index, SeqWhere& w) {
+// run backwards or leave the tensor are clamped: such a sequence is empty, nothing outside the tensor is touched.  `other` (or null): x0 =
+// other[b], x1 = other[b + two], fetched along with the starts.  Where the launch has more workgroups than the chip
+// holds at once, up to 64 sequences are gone through from the longest (rows, or rows + x0 where x0 counts keys in front of them: `two` 0) to
+// the shortest: it ends with its short tasks (eight chunks of up to 512 rows over up to 6000 keys: 223 -> 187 us; about 1 us of a small launch).
+struct SeqWhere { int b, tile, start, n, x0, x1; };
+__device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total, int mult, int rows, int index, const int32_t* other, int two, SeqWhere& w) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int b0 = 0; b0 < batch; b0 += 64) {
-    const int b = b0 + lane;
-    int s = 0, e = 0;
-    if (b < batch) { s = cu[b]; e = cu[b + 1]; }
+    int b = b0 + lane;
+    int s = 0, e = 0, x0 = 0, x1 = 0;
+    if (b < batch) {
+      s = cu[b]; e = cu[b + 1];
+      if (other) { x0 = other[b]; x1 = other[b + two]; }
+    }
     s = s < 0 ? 0 : (s > total ? total : s);
     e = e < s ? s : (e > total ? total : e);
-    const int n = e - s;
-    const int t = (int)(((long long)n * mult + rows - 1) / rows);
-    int x = t;                                             // inclusive scan over the 64 sequences
+    int n = e - s;
+    int t = (int)(((long long)n * mult + rows - 1) / rows);
+    if (gridDim.x > 512 && batch > 1 && batch <= 64) {       // ranks, then everything to the lane of its rank
+      const int key = b < batch ? n + (two ? 0 : x0) : -1;
+      int rank = 0;
+      for (int j = 0; j < batch; ++j) { const int k = __builtin_amdgcn_readlane(key, j); rank += (k > key || (k == key && j < lane)) ? 1 : 0; }
+      rank = b < batch ? rank : lane;
+      auto to = [&](int v) { return __builtin_amdgcn_ds_permute(rank << 2, v); };
+      b = to(b); s = to(s); n = to(n); t = to(t); x0 = to(x0); x1 = to(x1);
+    }
+    int x = t;                                               // inclusive scan over the 64 sequences
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
     const unsigned long long m = __builtin_amdgcn_ballot_w64(index < before + x);
     if (m) {
       const int src = __builtin_ctzll(m);
-      w.b = b0 + src;
-      w.tile = index - before - __shfl(x - t, src, 64);
-      w.start = __shfl(s, src, 64);
-      w.n = __shfl(n, src, 64);
-      w.b = __builtin_amdgcn_readfirstlane(w.b); w.tile = __builtin_amdgcn_readfirstlane(w.tile);
-      w.start = __builtin_amdgcn_readfirstlane(w.start); w.n = __builtin_amdgcn_readfirstlane(w.n);
+      w.tile = index - before - __builtin_amdgcn_readlane(x - t, src);
+      w.b = __builtin_amdgcn_readlane(b, src); w.start = __builtin_amdgcn_readlane(s, src); w.n = __builtin_amdgcn_readlane(n, src);
+      w.x0 = __builtin_amdgcn_readlane(x0, src); w.x1 = __builtin_amdgcn_readlane(x1, src);
       return true;
     }
-    before += __shfl(x, 63, 64);
+    before += __builtin_amdgcn_readlane(x, 63);
   }
   return false;
+}
+__device__ __forceinline__ void seq_clamp(int s, int e, int total, int& start, int& n) {
+  s = s < 0 ? 0 : (s > total ? total : s);
+  e = e < s ? s : (e > total ? total : e);
+  start = s; n = e - s;
 }
 // workgroup -> task: the hardware deals workgroups to the 8 XCDs in turn, the tasks of one XCD are to be neighbours (the same keys in its L2)
 __device__ __forceinline__ int seq_task(int id, int n) {

@@ -11,46 +11,60 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-template <typename T, int DP>
-__device__ __forceinline__ void tile_to_lds(const T* base, long long ld, int r0, int n, int dim, int i, char* tile, int lane, const void* zero) {
+// Rows of one head in memory, `ld` bytes apart; rows from n on read as zeros.  Whole tiles go by scalar addresses, the last one of a sequence
+// and heads narrower than the tile by an address in every lane (zeros where there is nothing).
+template <typename T, int DP> struct Rows {                    // (`first` is the same in set and fetch)
   typedef SeqTile<T, DP> L;
-  constexpr int kRowsOf = 64 / L::kChunks;
-  const int r = i * kRowsOf + lane / L::kChunks, c = (lane % L::kChunks) ^ (r & 7), row = r0 + r;
-  const void* p = (row < n && c * L::kPer < dim) ? (const void*)(base + row * ld + c * L::kPer) : zero;
-  seq_dma16(p, tile + i * 1024);
-}
-__device__ __forceinline__ void clamped(const int32_t* cu, int b, int total, int& start, int& n) {
-  int s = cu[b], e = cu[b + 1];
-  s = s < 0 ? 0 : (s > total ? total : s);
-  e = e < s ? s : (e > total ? total : e);
-  start = s; n = e - s;
-}
+  typedef SeqLanes<T, DP> W;
+  long long ld; int n, dim; const void* zero; bool plain; W w;
+  __device__ __forceinline__ void set(long long stride, int rows, int width, const void* zeros, int lane, int first) {
+    ld = stride * (int)sizeof(T); n = rows; dim = width; zero = zeros;
+    plain = width == DP && stride < (1 << 24);               // (a lane's offset in 32 bits)
+    w.set((unsigned)ld, lane, first);
+  }
+  // transfers first .. first + N - 1 of the tile of `rows` rows that starts at row r0 of `base`
+  template <int N> __device__ __forceinline__ void fetch(const void* base, int r0, int rows, int first, unsigned dst, int lane) const {
+    const char* p = (const char*)base + (r0 + first * W::kRowsOf) * ld;
+    if (plain && r0 + rows <= n) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) seq_dma16(p + i * W::kRowsOf * ld, w.at[i % W::kPeriod], dst + (first + i) * 1024);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = lane / L::kChunks, c = (lane % L::kChunks) ^ L::turn((first + i) * W::kRowsOf + r);
+      const char* q = p + (i * W::kRowsOf + r) * ld + c * 16;
+      seq_dma16(r0 + (first + i) * W::kRowsOf + r < n && c * L::kPer < dim ? (const void*)q : zero, dst + (first + i) * 1024);
+    }
+  }
+};
 
-// 128 query rows of one head.  Leaves delta and lse log2 e of its rows for the other kernel: delta [2][heads][rows_q].
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(const SeqGradArgs ga, const int tiles) {
+// 32 RG query rows of one head; KS key groups of waves, as in the forward kernel.  Leaves delta and lse log2 e of its rows for the other
+// kernel: delta [2][heads][rows_q].
+template <typename T, int DP, int RG, int KS>
+__global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(const SeqGradArgs ga, const int tiles) {
   typedef SeqTile<T, DP> L;
   typedef typename SeqVec<T>::v8 v8;
   const SeqArgs& a = ga.f;
-  constexpr int BN = 64, kTile = BN * L::kRow, kStage = 2 * kTile, kIssue = kTile / 4096;
+  constexpr int BM = 32 * RG, BN = RG == 4 ? 64 : 32, kTile = BN * L::kRow, kStage = 2 * kTile, kIssue = kTile / 1024 / RG, step = BN * KS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG, l31 = lane & 31, g = lane >> 5;
   const int group = a.heads / a.kv_heads;
   int task = seq_task(blockIdx.x, gridDim.x);
   const int hq = task % group; task /= group;
-  const int kvh = task / tiles; task = tiles - 1 - (task - kvh * tiles);
+  const int kvh = task / tiles; task -= kvh * tiles;
   SeqWhere w;
-  if (!seq_find(a.cu_q, a.batch, a.rows_q, 1, 128, task, w)) return;
+  if (!seq_find(a.cu_q, a.batch, a.rows_q, 1, BM, task, a.cu_k, 1, w)) return;
   int ks, nk;
-  clamped(a.cu_k, w.b, a.rows_k, ks, nk);
+  seq_clamp(w.x0, w.x1, a.rows_k, ks, nk);
   const int ahead = nk - w.n, head = kvh * group + hq;
-  const int r0 = w.tile * 128, row = r0 + 32 * wave + l31;
+  const int r0 = ((w.n + BM - 1) / BM - 1 - w.tile) * BM, row = r0 + 32 * rg + l31;
   const bool live = row < w.n;
   const int token = w.start + (live ? row : 0);
   auto seen = [&](int r) { const int x = a.causal ? ahead + r + 1 : nk; return x < 0 ? 0 : (x > nk ? nk : x); };
   const int limit = live ? seen(row) : 0;
-  const int last = (r0 + 128 < w.n ? r0 + 128 : w.n) - 1, some = seen(last);
-  const int wfirst = r0 + 32 * wave, wlast = (wfirst + 32 < w.n ? wfirst + 32 : w.n) - 1;
+  const int last = (r0 + BM < w.n ? r0 + BM : w.n) - 1, some = seen(last);
+  const int wfirst = r0 + 32 * rg, wlast = (wfirst + 32 < w.n ? wfirst + 32 : w.n) - 1;
   const int wall = wfirst < w.n ? seen(wfirst) : nk, wsome = wfirst < w.n ? seen(wlast) : 0;
 
   v8 qf[DP / 16], df[DP / 16];
@@ -62,9 +76,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(con
     for (int t = 0; t < DP / 16; ++t) {
       const int e0 = 16 * t + 8 * g;
       const bool ok = live && e0 < a.dim;
-      qf[t] = seq_load8<T>(qp + e0, ok);
-      df[t] = seq_load8<T>(dp + e0, ok);
-      const v8 o = seq_load8<T>(op + e0, ok);
+      qf[t] = seq_load8<T>(qp + e0, ok, a.zero);
+      df[t] = seq_load8<T>(dp + e0, ok, a.zero);
+      const v8 o = seq_load8<T>(op + e0, ok, a.zero);
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)df[t][e] * (float)o[e];
     }
@@ -74,7 +88,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(con
   if (live) {
     const long long at = (long long)head * a.rows_q + token, plane = (long long)a.heads * a.rows_q;
     lse2 = a.lse[at] * kLog2e;
-    if (g == 0) { ga.delta[at] = delta; ga.delta[plane + at] = lse2; }
+    if (g == 0 && kg == 0) { ga.delta[at] = delta; ga.delta[plane + at] = lse2; }
   }
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -83,25 +97,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(con
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   const float c = a.scale * kLog2e;
   const T *kb = (const T*)a.k + ks * a.ldk + (long long)kvh * a.dim, *vb = (const T*)a.v + ks * a.ldv + (long long)kvh * a.dim;
-  auto issue = [&](int k0, int stage) {
-    char* t = smem + stage * kStage;
-#pragma unroll
-    for (int i = 0; i < kIssue; ++i) {
-      tile_to_lds<T, DP>(kb, a.ldk, k0, nk, a.dim, wave * kIssue + i, t, lane, a.zero);
-      tile_to_lds<T, DP>(vb, a.ldv, k0, nk, a.dim, wave * kIssue + i, t + kTile, lane, a.zero);
+  char* base = smem + kg * 2 * kStage;
+  const unsigned lds = seq_lds(base);
+  Rows<T, DP> rk, rv;
+  rk.set(a.ldk, nk, a.dim, a.zero, lane, rg * kIssue); rv.set(a.ldv, nk, a.dim, a.zero, lane, rg * kIssue);
+  seq_settle(qf); seq_settle(df);
+  int k0 = (kg - KS) * BN, stage = 0;                        // (the first turn only fetches)
+  for (int kt = -step; kt < some; kt += step, k0 += step, stage ^= kStage) {
+    seq_dma_wait();
+    if (RG > 1) __syncthreads();
+    if (k0 + step < some) {
+      const unsigned t = lds + (stage ^ kStage);
+      rk.template fetch<kIssue>(kb, k0 + step, BN, rg * kIssue, t, lane);
+      rv.template fetch<kIssue>(vb, k0 + step, BN, rg * kIssue, t + kTile, lane);
     }
-  };
-  if (some > 0) issue(0, 0);
-  int stage = 0;
-  for (int k0 = 0; k0 < some; k0 += BN, stage ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (k0 + BN < some) issue(k0 + BN, stage ^ 1);
-    if (k0 >= wsome) continue;
-    const char *tk = smem + stage * kStage, *tv = tk + kTile;
+    if (kt < 0 || k0 >= some || k0 >= wsome) continue;
+    const char *tk = base + stage, *tv = tk + kTile;
     const bool masked = k0 + BN > wall;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < BN / 32; ++j) {
       f32x16 s, p;
 #pragma unroll
       for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
@@ -124,6 +138,27 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(con
       }
     }
   }
+  if (KS > 1) {                                              // the key groups' parts of the same rows, summed in the groups' order
+    __syncthreads();
+    constexpr int N = (DP / 32) * 16;
+    float* x = reinterpret_cast<float*>(smem) + lane;
+    if (kg > 0) {
+      float* y = x + ((kg - 1) * RG + rg) * N * 64;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[(16 * d + i) * 64] = acc[d][i];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+    for (int k = 0; k < KS - 1; ++k) {
+      const float* y = x + (k * RG + rg) * N * 64;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] += y[(16 * d + i) * 64];
+    }
+  }
   if (!live) return;
   T* dq = (T*)ga.dq + token * ga.lddq + (long long)head * a.dim;
 #pragma unroll
@@ -135,25 +170,26 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(con
     }
 }
 
-// 128 keys of one key / value head: 32 a wave, as the columns of S = Q K' and dP = dO V'; the query rows of every head of the group pass
-// through LDS in tiles of BQ.
-template <typename T, int DP, int BQ>
-__global__ void __launch_bounds__(256, 1) seq_dkv_kernel(const SeqGradArgs ga, const int tiles) {
+// 32 KG keys of one key / value head, 32 a wave, as the columns of S = Q K' and dP = dO V'; the query rows of every head of the group pass
+// through LDS in tiles of 32.  HG row groups of waves take the tiles in turn (each with buffers of its own) and their sums are joined at the
+// end: a sequence's first keys are seen by all of its rows in every head, one wave for them would outlast the rest of the launch.
+template <typename T, int DP, int KG, int HG>
+__global__ void __launch_bounds__(64 * KG * HG, 1) seq_dkv_kernel(const SeqGradArgs ga, const int tiles) {
   typedef SeqTile<T, DP> L;
   typedef typename SeqVec<T>::v8 v8;
   const SeqArgs& a = ga.f;
-  constexpr int kTile = BQ * L::kRow, kStage = 2 * kTile + 2 * BQ * 4, kIssue = kTile / 4096;
+  constexpr int BK = 32 * KG, BQ = 32, kTile = BQ * L::kRow, kStage = 2 * kTile + 256, kIssue = kTile / 1024 / KG;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave % KG, hg = wave / KG, l31 = lane & 31, g = lane >> 5;
   const int group = a.heads / a.kv_heads;
   int task = seq_task(blockIdx.x, gridDim.x);
   const int kvh = task / tiles; task -= kvh * tiles;         // (causal: the first keys of a sequence are seen by most rows: long ones first)
   SeqWhere w;
-  if (!seq_find(a.cu_k, a.batch, a.rows_k, 1, 128, task, w)) return;
+  if (!seq_find(a.cu_k, a.batch, a.rows_k, 1, BK, task, a.cu_q, 1, w)) return;
   int qs, nq;
-  clamped(a.cu_q, w.b, a.rows_q, qs, nq);
+  seq_clamp(w.x0, w.x1, a.rows_q, qs, nq);
   const int nk = w.n, ahead = nk - nq;
-  const int k0 = w.tile * 128, kw = k0 + 32 * wave, key = kw + l31;
+  const int k0 = w.tile * BK, kw = k0 + 32 * kg, key = kw + l31;
   const bool live = key < nk;
   v8 kf[DP / 16], vf[DP / 16];
   {
@@ -162,8 +198,8 @@ __global__ void __launch_bounds__(256, 1) seq_dkv_kernel(const SeqGradArgs ga, c
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
       const int e0 = 16 * t + 8 * g;
-      kf[t] = seq_load8<T>(kp + e0, live && e0 < a.dim);
-      vf[t] = seq_load8<T>(vp + e0, live && e0 < a.dim);
+      kf[t] = seq_load8<T>(kp + e0, live && e0 < a.dim, a.zero);
+      vf[t] = seq_load8<T>(vp + e0, live && e0 < a.dim, a.zero);
     }
   }
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -177,51 +213,54 @@ __global__ void __launch_bounds__(256, 1) seq_dkv_kernel(const SeqGradArgs ga, c
   first = first < 0 ? 0 : first / BQ * BQ;
   const int per = nq > first ? (nq - first + BQ - 1) / BQ : 0, total = per * group;
   const long long plane = (long long)a.heads * a.rows_q;
-  auto issue = [&](int it, int stage) {
-    const int h = kvh * group + it / per, q0 = first + it % per * BQ;
-    char* t = smem + stage * kStage;
-    const T *qb = (const T*)a.q + qs * a.ldq + (long long)h * a.dim, *db = (const T*)ga.dout + qs * ga.lddo + (long long)h * a.dim;
-#pragma unroll
-    for (int i = 0; i < kIssue; ++i) {
-      tile_to_lds<T, DP>(qb, a.ldq, q0, nq, a.dim, wave * kIssue + i, t, lane, a.zero);
-      tile_to_lds<T, DP>(db, ga.lddo, q0, nq, a.dim, wave * kIssue + i, t + kTile, lane, a.zero);
+  char* base = smem + hg * 2 * kStage;
+  const unsigned lds = seq_lds(base);
+  Rows<T, DP> rq, rd;
+  rq.set(a.ldq, nq, a.dim, a.zero, lane, kg * kIssue); rd.set(ga.lddo, nq, a.dim, a.zero, lane, kg * kIssue);
+  const char *qb = (const char*)((const T*)a.q + qs * a.ldq), *db = (const char*)((const T*)ga.dout + qs * ga.lddo);
+  seq_settle(kf); seq_settle(vf);
+  // tile `at` of head `h` of the group is next, r0 is the first row of this turn's; the first turn only fetches
+  int h = 0, at = hg, r0 = 0, stage = 0;
+  while (per > 0 && at >= per) { at -= per; ++h; }
+  for (int it = hg - HG, turn = -HG; turn < total; turn += HG, it += HG, stage ^= kStage) {       // (every group as often: the barrier is everybody's)
+    seq_dma_wait();
+    if (KG > 1) __syncthreads();
+    const int row = r0;
+    if (it + HG < total) {
+      const unsigned t = lds + (stage ^ kStage);
+      const int hd = kvh * group + h;
+      const long long ho = (long long)hd * a.dim * (int)sizeof(T);
+      r0 = first + at * BQ;
+      rq.template fetch<kIssue>(qb + ho, r0, BQ, kg * kIssue, t, lane);
+      rd.template fetch<kIssue>(db + ho, r0, BQ, kg * kIssue, t + kTile, lane);
+      if (kg == 0) {                                         // delta, then lse of the tile's rows: four bytes a lane
+        const float* x = ga.delta + (g ? plane : 0) + (long long)hd * a.rows_q + qs + r0 + l31;
+        seq_dma4(r0 + l31 < nq ? (const void*)x : a.zero, t + 2 * kTile);
+      }
+      at += HG;
+      while (at >= per) { at -= per; ++h; }
     }
-    if (wave < 2 && lane < BQ) {                             // delta and lse of the rows: four bytes a lane
-      const float* x = ga.delta + wave * plane + (long long)h * a.rows_q + qs + q0 + lane;
-      const void* p = q0 + lane < nq ? (const void*)x : a.zero;
-      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)(t + 2 * kTile + wave * BQ * 4), 4, 0, 0);
-    }
-  };
-  if (total > 0) issue(0, 0);
-  int stage = 0;
-  for (int it = 0; it < total; ++it, stage ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (it + 1 < total) issue(it + 1, stage ^ 1);
-    const int q0 = first + it % per * BQ;
-    const char *tq = smem + stage * kStage, *td = tq + kTile;
+    if (turn < 0 || it >= total || (a.causal && row + 31 + ahead < kw)) continue;        // (or none of these rows sees the wave's keys)
+    const char *tq = base + stage, *td = tq + kTile;
     const float *delta = reinterpret_cast<const float*>(td + kTile), *lse2 = delta + BQ;
-#pragma unroll
-    for (int j = 0; j < BQ / 32; ++j) {
-      const int r0 = q0 + 32 * j;
-      if (a.causal && r0 + 31 + ahead < kw) continue;        // (wave-uniform) none of these rows sees the wave's keys
+    {
       f32x16 s, p;
 #pragma unroll
       for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
-        s = seq_mma(seq_row<T, DP>(tq, 32 * j + l31, 2 * t + g), kf[t], s);
-        p = seq_mma(seq_row<T, DP>(td, 32 * j + l31, 2 * t + g), vf[t], p);
+        s = seq_mma(seq_row<T, DP>(tq, l31, 2 * t + g), kf[t], s);
+        p = seq_mma(seq_row<T, DP>(td, l31, 2 * t + g), vf[t], p);
       }
-      const bool masked = a.causal && r0 + ahead < kw + 31;
+      const bool masked = a.causal && row + ahead < kw + 31;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const sq_f4 ls = *reinterpret_cast<const sq_f4*>(lse2 + 32 * j + 8 * q + 4 * g), de = *reinterpret_cast<const sq_f4*>(delta + 32 * j + 8 * q + 4 * g);
+        const sq_f4 ls = *reinterpret_cast<const sq_f4*>(lse2 + 8 * q + 4 * g), de = *reinterpret_cast<const sq_f4*>(delta + 8 * q + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * q + e;
           float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[e])), y = x * (p[i] - de[e]);
-          if (masked) { const bool ok = key <= r0 + 8 * q + 4 * g + e + ahead; x = ok ? x : 0.f; y = ok ? y : 0.f; }
+          if (masked) { const bool ok = key <= row + 8 * q + 4 * g + e + ahead; x = ok ? x : 0.f; y = ok ? y : 0.f; }
           s[i] = x; p[i] = y;
         }
       }
@@ -230,11 +269,37 @@ __global__ void __launch_bounds__(256, 1) seq_dkv_kernel(const SeqGradArgs ga, c
         const v8 pf = seq_pack<T>(s, t), sf = seq_pack<T>(p, t);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = seq_mma(seq_col<T, DP>(td, 32 * j + 16 * t, d, lane), pf, dv[d]);
-          dk[d] = seq_mma(seq_col<T, DP>(tq, 32 * j + 16 * t, d, lane), sf, dk[d]);
+          dv[d] = seq_mma(seq_col<T, DP>(td, 16 * t, d, lane), pf, dv[d]);
+          dk[d] = seq_mma(seq_col<T, DP>(tq, 16 * t, d, lane), sf, dk[d]);
         }
       }
     }
+  }
+  if (HG > 1) {                                              // the row groups' sums, in their order: dK, then dV through the same buffer
+    constexpr int N = (DP / 32) * 16;
+    float* x = reinterpret_cast<float*>(smem) + lane;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
+      if (hg > 0) {
+        float* y = x + ((hg - 1) * KG + kg) * N * 64;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[(16 * d + i) * 64] = half ? dv[d][i] : dk[d][i];
+      }
+      __syncthreads();
+      if (hg == 0) {
+        for (int k = 0; k < HG - 1; ++k) {
+          const float* y = x + (k * KG + kg) * N * 64;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { if (half) dv[d][i] += y[(16 * d + i) * 64]; else dk[d][i] += y[(16 * d + i) * 64]; }
+        }
+      }
+    }
+    if (hg > 0) return;
   }
   if (!live) return;
   T *pk = (T*)ga.dk + (w.start + key) * ga.lddk + (long long)kvh * a.dim, *pv = (T*)ga.dv + (w.start + key) * ga.lddv + (long long)kvh * a.dim;
@@ -250,37 +315,46 @@ __global__ void __launch_bounds__(256, 1) seq_dkv_kernel(const SeqGradArgs ga, c
     }
 }
 
-template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, hipStream_t s) {
-  typedef SeqTile<T, DP> L;
-  static int done_q[kMaxDevices], done_kv[kMaxDevices];
+template <typename T, int DP, int RG, int KS> hipError_t grad_q(const SeqGradArgs& a, hipStream_t s) {
+  static int done[kMaxDevices];
+  constexpr int BN = RG == 4 ? 64 : 32, tiles_lds = KS * 4 * BN * SeqTile<T, DP>::kRow, join = (KS - 1) * RG * (DP / 32) * 16 * 256, lds = tiles_lds > join ? tiles_lds : join;
+  static_assert(lds <= 160 * 1024, "LDS");
+  opt_in_dynamic_lds((const void*)seq_dq_kernel<T, DP, RG, KS>, lds, done);
   const SeqArgs& f = a.f;
-  if (f.rows_q > 0) {
-    constexpr int lds = 2 * 2 * 64 * L::kRow;
-    opt_in_dynamic_lds((const void*)seq_dq_kernel<T, DP>, lds, done_q);
-    const int tiles = f.rows_q / 128 + (f.batch < f.rows_q ? f.batch : f.rows_q);
-    const long long grid = (long long)tiles * f.heads;
-    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    vnr_launch(seq_dq_kernel<T, DP>, dim3((unsigned)grid), dim3(256), lds, s, a, tiles);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (f.rows_k > 0) {
-    constexpr int BQ = 64, lds = 2 * (2 * BQ * L::kRow + 8 * BQ);
-    static_assert(lds <= 160 * 1024, "LDS");
-    opt_in_dynamic_lds((const void*)seq_dkv_kernel<T, DP, BQ>, lds, done_kv);
-    const int tiles = f.rows_k / 128 + (f.batch < f.rows_k ? f.batch : f.rows_k);
-    const long long grid = (long long)tiles * f.kv_heads;
-    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    vnr_launch(seq_dkv_kernel<T, DP, BQ>, dim3((unsigned)grid), dim3(256), lds, s, a, tiles);
-  }
+  const int tiles = f.rows_q / (32 * RG) + (f.batch < f.rows_q ? f.batch : f.rows_q);
+  const long long grid = (long long)tiles * f.heads;
+  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  vnr_launch(seq_dq_kernel<T, DP, RG, KS>, dim3((unsigned)grid), dim3(64 * RG * KS), lds, s, a, tiles);
   return hipGetLastError();
 }
-template <typename T> hipError_t grad(const SeqGradArgs& a, hipStream_t s) { return a.f.dim <= 64 ? grad<T, 64>(a, s) : grad<T, 128>(a, s); }
+template <typename T, int DP, int KG, int HG> hipError_t grad_kv(const SeqGradArgs& a, hipStream_t s) {
+  static int done[kMaxDevices];
+  constexpr int tiles_lds = HG * 2 * (2 * 32 * SeqTile<T, DP>::kRow + 256), join = (HG - 1) * KG * (DP / 32) * 16 * 256, lds = tiles_lds > join ? tiles_lds : join;
+  static_assert(lds <= 160 * 1024, "LDS");
+  opt_in_dynamic_lds((const void*)seq_dkv_kernel<T, DP, KG, HG>, lds, done);
+  const SeqArgs& f = a.f;
+  const int tiles = f.rows_k / (32 * KG) + (f.batch < f.rows_k ? f.batch : f.rows_k);
+  const long long grid = (long long)tiles * f.kv_heads;
+  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  vnr_launch(seq_dkv_kernel<T, DP, KG, HG>, dim3((unsigned)grid), dim3(64 * KG * HG), lds, s, a, tiles);
+  return hipGetLastError();
+}
+template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, int cus, hipStream_t s) {
+  hipError_t e = hipSuccess;
+  const SeqArgs& f = a.f;
+  // 128 query rows a workgroup where that makes two for each compute unit, else 64 (32 utterances of up to 400 rows, 4 heads, f32: both kernels
+  // 156 / 128 us with 128 / 64; 4 sequences of up to 2048, 32 heads of 128, bf16: 281 / 295)
+  const long long wgs = ((long long)f.rows_q / 128 + (f.batch < f.rows_q ? f.batch : f.rows_q)) * f.heads;
+  if (f.rows_q > 0) e = wgs >= 2LL * cus ? grad_q<T, DP, 4, 1>(a, s) : grad_q<T, DP, 2, 2>(a, s);
+  if (e != hipSuccess || f.rows_k == 0) return e;
+  return grad_kv<T, DP, 2, 2>(a, s);
+}
+template <typename T> hipError_t grad(const SeqGradArgs& a, int cus, hipStream_t s) { return a.f.dim <= 64 ? grad<T, 64>(a, cus, s) : grad<T, 128>(a, cus, s); }
 }  // namespace
 
-hipError_t launch_seq_grad(const SeqGradArgs& a, hipStream_t s) {
-  if (a.f.dtype == SEQ_F32) return grad<float>(a, s);
-  if (a.f.dtype == SEQ_F16) return grad<_Float16>(a, s);
-  return grad<sq_bf16>(a, s);
+hipError_t launch_seq_grad(const SeqGradArgs& a, int cus, hipStream_t s) {
+  if (a.f.dtype == SEQ_F32) return grad<float>(a, cus, s);
+  if (a.f.dtype == SEQ_F16) return grad<_Float16>(a, cus, s);
+  return grad<sq_bf16>(a, cus, s);
 }
 }  // namespace vnr
