@@ -547,6 +547,75 @@ def test_paged_attention_reads_absent_pages_as_zeros(eng):
     close(out.numpy(), want["out"], "out")
 
 
+def prefix(q, k, v, limit, scale):
+    """Row by row over the keys it sees and no other: what is behind them may be anything."""
+    out = np.zeros((q.shape[0], v.shape[1]))
+    with np.errstate(invalid="ignore"):
+        for i, n in enumerate(limit):
+            if n > 0:
+                x = k[:n] @ q[i] * scale
+                p = np.exp(x - x.max())
+                out[i] = (p / p.sum()) @ v[:n]
+    return out
+
+
+TAINTS = [
+    # what, sequence's rows, its keys in front (a cache), head width; places (row or None = all channels, channel)
+    ("v", 90, 0, 64, [(40, None)]),
+    ("v", 200, 0, 128, [(0, 5), (131, 9), (140, None)]),
+    ("v", 70, 0, 64, [(69, None)]),
+    ("k", 100, 0, 128, [(33, None), (99, None)]),
+    ("v", 130, 70, 64, [(75, 3), (150, None)]),
+    ("v", 50, 300, 128, [(320, None), (349, 0)]),
+    ("k", 3, 61, 64, [(62, None)]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("number", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("case", TAINTS, ids=[str(i) for i in range(len(TAINTS))])
+def test_later_keys_that_are_not_finite_reach_no_earlier_row(eng, case, number, kind):
+    """An infinity or a NaN in a key or value that a row does not see leaves that row as it is, whichever tile it shares with others that do
+    see it; the rows that see it get what the arithmetic gives.  Small and large launches take different kernels: 1 and 80 heads."""
+    what, n, ctx, D, places = case
+    r = np.random.default_rng(n + ctx)
+    total = n + ctx
+    k, v = normal(r, kind, total, 1, D), normal(r, kind, total, 1, D)
+    for row, ch in places:
+        (v if what == "v" else k)[row, 0, slice(None) if ch is None else ch] = store(np.float32([number]), kind)[0]
+    for H in (1, 80) if ctx == 0 else (1, 4, 40):
+        q = normal(r, kind, n, H, D)
+        limit = ctx + np.arange(n) + 1
+        if ctx == 0:
+            out, _ = sequence.packed_attention(eng, eng.to_device(q), eng.to_device(k), eng.to_device(v), eng.to_device(starts([n])))
+        else:
+            P = 16
+            table, pages = layout(r, [total], P)
+            kc, vc = np.zeros((pages, 1, P, D), k.dtype), np.zeros((pages, 1, P, D), k.dtype)
+            for p in range(total):
+                kc[table[0, p // P], :, p % P], vc[table[0, p // P], :, p % P] = k[p], v[p]
+            out = sequence.PagedCache(eng, eng.to_device(kc), eng.to_device(vc)).attend(
+                eng.to_device(q), eng.to_device(starts([n])), eng.to_device(np.int32([ctx])), eng.to_device(table), n, total)
+        got = value(out.numpy())
+        clean_k, clean_v = value(k)[:, 0], value(v)[:, 0]
+        for h in (0, H - 1):
+            want = prefix(value(q)[:, h], clean_k, clean_v, limit, np.float64(np.float32(D ** -0.5)))
+            fine = np.isfinite(want)
+            first = min(p for p, _ in places)
+            assert np.isfinite(got[:max(0, first - ctx), h]).all()                  # rows in front of all of them
+            if what == "v":                                                         # (a logit that is not finite makes its row's sums so, one way or another)
+                assert (np.isfinite(got[:, h]) == fine).all()
+                # an infinity may come out as NaN: a weight below 2^-25 of the row's largest is 0 in float16 (below 2^-126 in the others),
+                # and 0 times infinity is NaN; it comes out as no other infinity
+                inf = np.isinf(want) & np.isinf(got[:, h])
+                assert (got[:, h][inf] == want[inf]).all()
+            u = KINDS[kind][1]
+            ok = fine & np.isfinite(got[:, h])
+            # (8 u of the values' size is wide of the derived bounds above: what is looked for here is a reach, not a rounding)
+            assert np.abs(got[:, h][ok] - want[ok]).max(initial=0) <= 8 * u + 1e-4, (H, h)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_prompt_then_chunks_then_single_rows(eng, kind):

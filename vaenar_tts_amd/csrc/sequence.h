@@ -82,38 +82,54 @@ template <typename T, int DP> struct SeqTile {
   }
   static __device__ __forceinline__ int at(int r, int c) { return r * kRow + ((c ^ turn(r)) << 4); }
 };
-// operand with rows along the lanes: elements 8 u .. 8 u + 7 of row r
-template <typename T, int DP>
-__device__ __forceinline__ typename SeqVec<T>::v8 seq_row(const char* tile, int r, int u) {
+// Where a lane reads its operands in a tile (bytes of LDS).  row: lane (r = lane & 31, g = lane >> 5) reads elements 16 t + 8 g .. + 7 of row r;
+// col: column 32 cb + r, k-slot (g, e) = row r0 + (e & 3) + 4 g + 8 (e >> 2) -- the order in which a product's registers 8 t .. 8 t + 7 hold
+// its rows, so the other operand of the next product comes straight out of them.  Everything that varies inside a tile is an exclusive or of
+// the address with a constant (turn() again), so two registers do for all of a tile's reads -- as long as the compiler does not keep every one
+// of the addresses: seq_at() hides the sum of tile and lane from it, once a tile.
+template <typename T, int DP> struct SeqReads {
+  typedef SeqTile<T, DP> L;
+  unsigned row, col;
+  __device__ __forceinline__ void set(int lane) {
+    const int r = lane & 31, g = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, q = 4 * g + (i >> 2);         // transposing reads: a 16-lane group reads a 4 x 16 block, lane i gets column i
+      row = L::at(r, g);
+      col = L::at(q, ((lane >> 4) & 1) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+    } else {
+      row = L::at(r, 2 * g);
+      col = L::at(4 * g, r >> 2) + (r & 3) * 4;
+    }
+  }
+};
+__device__ __forceinline__ unsigned seq_at(unsigned tile, unsigned lane) {
+  unsigned x = tile + lane;
+  asm volatile("" : "+v"(x));
+  return x;
+}
+template <typename V> __device__ __forceinline__ V seq_ds(unsigned at) { return *(const __attribute__((address_space(3))) V*)at; }
+// at: seq_at(tile, reads.row); rows r0 .. r0 + 31 of the tile
+template <typename T, int DP> __device__ __forceinline__ typename SeqVec<T>::v8 seq_row(unsigned at, int r0, int t) {
   typedef SeqTile<T, DP> L;
   if constexpr (sizeof(T) == 2) {
-    return *reinterpret_cast<const typename SeqVec<T>::v8*>(tile + L::at(r, u));
+    return seq_ds<typename SeqVec<T>::v8>((at ^ (t << 5)) + r0 * L::kRow);
   } else {
-    const sq_f4 a = *reinterpret_cast<const sq_f4*>(tile + L::at(r, 2 * u)), b = *reinterpret_cast<const sq_f4*>(tile + L::at(r, 2 * u + 1));
+    const sq_f4 a = seq_ds<sq_f4>((at ^ (t << 6)) + r0 * L::kRow), b = seq_ds<sq_f4>((at ^ (t << 6) ^ 16) + r0 * L::kRow);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
-// operand with columns along the lanes: column 32 cb + (lane & 31), k-slot (g, e) = row r0 + (e & 3) + 4 g + 8 (e >> 2) -- the order in which
-// a product's registers 8 t .. 8 t + 7 hold its rows, so the other operand of the next product comes straight out of them.  16 bits: two
-// transposing LDS reads (a 16-lane group reads a 4 x 16 block, lane i gets column i).
-template <typename T, int DP>
-__device__ __forceinline__ typename SeqVec<T>::v8 seq_col(const char* tile, int r0, int cb, int lane) {
+// at: seq_at(tile, reads.col); r0: a multiple of 16
+template <typename T, int DP> __device__ __forceinline__ typename SeqVec<T>::v8 seq_col(unsigned at, int r0, int cb) {
   typedef SeqTile<T, DP> L;
-  const int g = lane >> 5;
   if constexpr (sizeof(T) == 2) {
-    const int i = lane & 15, r = r0 + 4 * g + (i >> 2), c = cb * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
     typedef __attribute__((address_space(3))) sq_s4* lp;
-    const sq_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(tile + L::at(r, c) + (i & 1) * 8));
-    const sq_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(tile + L::at(r + 8, c) + (i & 1) * 8));
+    const sq_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)((at ^ (cb << 6)) + r0 * L::kRow));
+    const sq_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)((at ^ (cb << 6) ^ 32) + (r0 + 8) * L::kRow));
     return __builtin_bit_cast(typename SeqVec<T>::v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   } else {
     sq_f8 v;
-    const int d = 32 * cb + (lane & 31);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int r = r0 + 4 * g + (e & 3) + 8 * (e >> 2);
-      v[e] = *reinterpret_cast<const float*>(tile + L::at(r, d >> 2) + (d & 3) * 4);
-    }
+    for (int e = 0; e < 8; ++e) v[e] = seq_ds<float>((at ^ (cb << 7) ^ ((e & 3) << 6) ^ ((e >> 2) << 5)) + (r0 + (e & 3) + 8 * (e >> 2)) * L::kRow);
     return v;
   }
 }
@@ -124,6 +140,51 @@ template <typename T> __device__ __forceinline__ typename SeqVec<T>::v8 seq_pack
   for (int e = 0; e < 8; ++e) v[e] = x[8 * t + e];
   if constexpr (sizeof(T) == 4) return v; else return __builtin_convertvector(v, typename SeqVec<T>::v8);
 }
+// the same with what the rounding left, rounded in turn: twice the bits for one product more
+template <typename T> __device__ __forceinline__ typename SeqVec<T>::v8 seq_pack(const f32x16& x, int t, typename SeqVec<T>::v8& rest) {
+  static_assert(sizeof(T) == 2, "32 bits leave nothing");
+  sq_f8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = x[8 * t + e];
+  typename SeqVec<T>::v8 r = __builtin_convertvector(v, typename SeqVec<T>::v8);
+  sq_f4 bits = __builtin_bit_cast(sq_f4, r);
+  asm("" : "+v"(bits));                                      // one rounding for both uses
+  r = __builtin_bit_cast(typename SeqVec<T>::v8, bits);
+  rest = __builtin_convertvector(v - __builtin_convertvector(r, sq_f8), typename SeqVec<T>::v8);
+  return r;
+}
+// Values that are not finite in a tile whose keys some row does not see: 0 times them would reach that row.  seq_tainted: does the tile hold any
+// (threads first, first + step, ... take its 16-byte chunks)?
+template <typename T, int DP, int ROWS> __device__ __forceinline__ bool seq_tainted(const char* tile, int first, int step) {
+  unsigned top = 0;
+  for (int q = first; q < ROWS * SeqTile<T, DP>::kChunks; q += step) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    const u4 x = *reinterpret_cast<const u4*>(tile + q * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned hi = sizeof(T) == 4 ? x[e] & 0x7fffffffu : x[e] & 0x7fff0000u, lo = sizeof(T) == 4 ? 0u : (x[e] << 16) & 0x7fff0000u;
+      top = top > hi ? top : hi; top = top > lo ? top : lo;
+    }
+  }
+  const unsigned limit = __is_same(T, _Float16) ? 0x7c000000u : 0x7f800000u;
+  return __builtin_amdgcn_ballot_w64(top >= limit) != 0;
+}
+// They become zeros in the tile, and what[0 / 1 / 2][channel] the first key (k0: the tile's first) with plus infinity / minus infinity / no number
+// there: a row sees a prefix of the keys, so it sees one of them if and only if it sees the first.
+template <typename T, int DP, int ROWS> __device__ __forceinline__ void seq_apart(char* tile, int* what, int k0, int first, int step) {
+  typedef SeqTile<T, DP> L;
+  for (int q = first; q < ROWS * L::kChunks; q += step) {
+    const int r = q / L::kChunks, c = (q % L::kChunks) ^ L::turn(r);
+    T* x = reinterpret_cast<T*>(tile + q * 16);
+    for (int e = 0; e < L::kPer; ++e) {
+      const float v = (float)x[e];
+      if (__builtin_fabsf(v) < __builtin_inff()) continue;
+      atomicMin(what + (v != v ? 2 : v > 0.f ? 0 : 1) * DP + c * L::kPer + e, k0 + r);
+      x[e] = (T)0.f;
+    }
+  }
+}
+
 // elements 8 u .. 8 u + 7 of a row in memory, zeros where `ok` is false (read from `zero`: no branch)
 template <typename T> __device__ __forceinline__ typename SeqVec<T>::v8 seq_load8(const T* p, bool ok, const void* zero) {
   return *reinterpret_cast<const typename SeqVec<T>::v8*>(ok ? (const void*)p : zero);
@@ -173,18 +234,17 @@ template <int left = 0> __device__ __forceinline__ void seq_dma_wait() { asm vol
 // every LDS read of the wave has been answered: what it read from may be overwritten
 __device__ __forceinline__ void seq_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// The offsets of a wave's lanes in a transfer of 64 chunks (kRowsOf rows, `ld` bytes apart): they repeat every kPeriod transfers
+// The offsets of a wave's lanes in its transfers of 64 chunks (kRowsOf rows, `ld` bytes apart, ld a multiple of a tile's row): turn() of a sum of
+// rows without common bits is the exclusive or of their turns, and what a transfer's first row adds stays inside the row.  One register.
 template <typename T, int DP> struct SeqLanes {
   typedef SeqTile<T, DP> L;
-  static constexpr int kRowsOf = 64 / L::kChunks, kPeriod = 16 / kRowsOf;
-  unsigned at[kPeriod];
-  __device__ __forceinline__ void set(unsigned ld, int lane, int first) {         // first: the wave's first transfer of a tile
-#pragma unroll
-    for (int i = 0; i < kPeriod; ++i) {
-      const int r = lane / L::kChunks;
-      at[i] = r * ld + (((lane % L::kChunks) ^ L::turn((first + i) * kRowsOf + r)) << 4);
-    }
+  static constexpr int kRowsOf = 64 / L::kChunks;
+  unsigned base;
+  __device__ __forceinline__ void set(unsigned ld, int lane, int first) {      // first: the wave's first transfer of a tile, a power of two's multiple of its count
+    const int r = lane / L::kChunks;
+    base = r * ld + (((lane % L::kChunks) ^ L::turn(r) ^ L::turn(first * kRowsOf)) << 4);
   }
+  __device__ __forceinline__ unsigned at(int i) const { return base ^ (unsigned)(L::turn(i * kRowsOf) << 4); }       // of the wave's i-th
 };
 // a load through the scalar cache: `p` is the same for the wave and nobody writes there during the kernel
 __device__ __forceinline__ int seq_scalar(const int32_t* p) {

@@ -19,7 +19,7 @@ template <typename T, int DP> struct Rows {                    // (`first` is th
   long long ld; int n, dim; const void* zero; bool plain; W w;
   __device__ __forceinline__ void set(long long stride, int rows, int width, const void* zeros, int lane, int first) {
     ld = stride * (int)sizeof(T); n = rows; dim = width; zero = zeros;
-    plain = width == DP && stride < (1 << 24);               // (a lane's offset in 32 bits)
+    plain = width == DP && stride < (1 << 24) && !(ld % L::kRow);      // (SeqLanes; a lane's offset in 32 bits)
     w.set((unsigned)ld, lane, first);
   }
   // transfers first .. first + N - 1 of the tile of `rows` rows that starts at row r0 of `base`
@@ -27,9 +27,10 @@ template <typename T, int DP> struct Rows {                    // (`first` is th
     const char* p = (const char*)base + (r0 + first * W::kRowsOf) * ld;
     if (plain && r0 + rows <= n) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) seq_dma16(p + i * W::kRowsOf * ld, w.at[i % W::kPeriod], dst + (first + i) * 1024);
+      for (int i = 0; i < N; ++i) seq_dma16(p + i * W::kRowsOf * ld, w.at(i), dst + (first + i) * 1024);
       return;
     }
+    asm volatile("" : "+v"(lane));                           // (opaque: or what follows from it is kept in registers all the way)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = lane / L::kChunks, c = (lane % L::kChunks) ^ L::turn((first + i) * W::kRowsOf + r);
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
   typedef typename SeqVec<T>::v8 v8;
   const SeqArgs& a = ga.f;
   constexpr int BM = 32 * RG, BN = RG == 4 ? 64 : 32, kTile = BN * L::kRow, kStage = 2 * kTile, kIssue = kTile / 1024 / RG, step = BN * KS;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(512))) char smem[];         // (SeqReads: tiles start at multiples of their row)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG, l31 = lane & 31, g = lane >> 5;
   const int group = a.heads / a.kv_heads;
   int task = seq_task(blockIdx.x, gridDim.x);
@@ -97,8 +98,9 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   const float c = a.scale * kLog2e;
   const T *kb = (const T*)a.k + ks * a.ldk + (long long)kvh * a.dim, *vb = (const T*)a.v + ks * a.ldv + (long long)kvh * a.dim;
-  char* base = smem + kg * 2 * kStage;
-  const unsigned lds = seq_lds(base);
+  const unsigned lds = seq_lds(smem) + kg * 2 * kStage;
+  SeqReads<T, DP> reads;
+  reads.set(lane);
   Rows<T, DP> rk, rv;
   rk.set(a.ldk, nk, a.dim, a.zero, lane, rg * kIssue); rv.set(a.ldv, nk, a.dim, a.zero, lane, rg * kIssue);
   seq_settle(qf); seq_settle(df);
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
       rv.template fetch<kIssue>(vb, k0 + step, BN, rg * kIssue, t + kTile, lane);
     }
     if (kt < 0 || k0 >= some || k0 >= wsome) continue;
-    const char *tk = base + stage, *tv = tk + kTile;
+    const unsigned tk = seq_at(lds + stage, reads.row), tc = seq_at(lds + stage, reads.col);
     const bool masked = k0 + BN > wall;
 #pragma unroll
     for (int j = 0; j < BN / 32; ++j) {
@@ -121,8 +123,8 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
       for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
-        s = seq_mma(seq_row<T, DP>(tk, 32 * j + l31, 2 * t + g), qf[t], s);
-        p = seq_mma(seq_row<T, DP>(tv, 32 * j + l31, 2 * t + g), df[t], p);
+        s = seq_mma(seq_row<T, DP>(tk, 32 * j, t), qf[t], s);
+        p = seq_mma(seq_row<T, DP>(tk, BN + 32 * j, t), df[t], p);         // (V lies behind K)
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2)) * (p[i] - delta);
@@ -132,9 +134,20 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const v8 ds = seq_pack<T>(s, t);
+        if constexpr (sizeof(T) == 2) {
+          v8 rest;
+          const v8 ds = seq_pack<T>(s, t, rest);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[d] = seq_mma(seq_col<T, DP>(tk, 32 * j + 16 * t, d, lane), ds, acc[d]);
+          for (int d = 0; d < DP / 32; ++d) {
+            const v8 k = seq_col<T, DP>(tc, 32 * j + 16 * t, d);
+            acc[d] = seq_mma(k, ds, acc[d]);
+            acc[d] = seq_mma(k, rest, acc[d]);
+          }
+        } else {
+          const v8 ds = seq_pack<T>(s, t);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) acc[d] = seq_mma(seq_col<T, DP>(tc, 32 * j + 16 * t, d), ds, acc[d]);
+        }
       }
     }
   }
@@ -174,12 +187,12 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
 // through LDS in tiles of 32.  HG row groups of waves take the tiles in turn (each with buffers of its own) and their sums are joined at the
 // end: a sequence's first keys are seen by all of its rows in every head, one wave for them would outlast the rest of the launch.
 template <typename T, int DP, int KG, int HG>
-__global__ void __launch_bounds__(64 * KG * HG, 1) seq_dkv_kernel(const SeqGradArgs ga, const int tiles) {
+__global__ void __launch_bounds__(64 * KG * HG, sizeof(T) == 2 ? 2 : 1) seq_dkv_kernel(const SeqGradArgs ga, const int tiles) {
   typedef SeqTile<T, DP> L;
   typedef typename SeqVec<T>::v8 v8;
   const SeqArgs& a = ga.f;
-  constexpr int BK = 32 * KG, BQ = 32, kTile = BQ * L::kRow, kStage = 2 * kTile + 256, kIssue = kTile / 1024 / KG;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int BK = 32 * KG, BQ = 32, kTile = BQ * L::kRow, kStage = 2 * kTile + (L::kRow > 256 ? 512 : 256), kIssue = kTile / 1024 / KG;
+  extern __shared__ __attribute__((aligned(512))) char smem[];         // (SeqReads: tiles start at multiples of their row)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave % KG, hg = wave / KG, l31 = lane & 31, g = lane >> 5;
   const int group = a.heads / a.kv_heads;
   int task = seq_task(blockIdx.x, gridDim.x);
@@ -213,67 +226,92 @@ __global__ void __launch_bounds__(64 * KG * HG, 1) seq_dkv_kernel(const SeqGradA
   first = first < 0 ? 0 : first / BQ * BQ;
   const int per = nq > first ? (nq - first + BQ - 1) / BQ : 0, total = per * group;
   const long long plane = (long long)a.heads * a.rows_q;
-  char* base = smem + hg * 2 * kStage;
-  const unsigned lds = seq_lds(base);
+  const unsigned lds = seq_lds(smem) + hg * 2 * kStage;
   Rows<T, DP> rq, rd;
   rq.set(a.ldq, nq, a.dim, a.zero, lane, kg * kIssue); rd.set(ga.lddo, nq, a.dim, a.zero, lane, kg * kIssue);
   const char *qb = (const char*)((const T*)a.q + qs * a.ldq), *db = (const char*)((const T*)ga.dout + qs * ga.lddo);
   seq_settle(kf); seq_settle(vf);
-  // tile `at` of head `h` of the group is next, r0 is the first row of this turn's; the first turn only fetches
-  int h = 0, at = hg, r0 = 0, stage = 0;
+  // ---- one tile of rows: the two products, the weights and their gradients, what they add to dV and dK ----------------------------------------
+  f32x16 s, p;
+  SeqReads<T, DP> reads;
+  reads.set(lane);
+  auto products = [&](unsigned tile) {
+    const unsigned at = seq_at(tile, reads.row);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      s = seq_mma(seq_row<T, DP>(at, 0, t), kf[t], s);
+      p = seq_mma(seq_row<T, DP>(at, BQ, t), vf[t], p);      // (dO lies behind Q)
+    }
+  };
+  auto weights = [&](unsigned tile) {
+    const unsigned at = seq_at(tile, 16 * g);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const sq_f4 de = seq_ds<sq_f4>(at + 2 * kTile + 32 * q), ls = seq_ds<sq_f4>(at + 2 * kTile + 4 * BQ + 32 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * q + e;
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[e]));
+        p[i] = x * (p[i] - de[e]);
+        s[i] = x;
+      }
+    }
+  };
+  auto masks = [&](int row) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const bool ok = key <= row + 8 * (i >> 2) + 4 * g + (i & 3) + ahead;
+      s[i] = ok ? s[i] : 0.f; p[i] = ok ? p[i] : 0.f;
+    }
+  };
+  auto sums = [&](unsigned tile) {
+    const unsigned at = seq_at(tile, reads.col);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      v8 rest = {};
+      const v8 pf = seq_pack<T>(s, t);
+      v8 sf;
+      if constexpr (sizeof(T) == 2) sf = seq_pack<T>(p, t, rest); else sf = seq_pack<T>(p, t);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        dv[d] = seq_mma(seq_col<T, DP>(at, BQ + 16 * t, d), pf, dv[d]);
+        const v8 q = seq_col<T, DP>(at, 16 * t, d);
+        dk[d] = seq_mma(q, sf, dk[d]);
+        if constexpr (sizeof(T) == 2) dk[d] = seq_mma(q, rest, dk[d]);
+      }
+    }
+  };
+  // tile `at` of head `h` of the group is fetched next
+  int h = 0, at = hg;
   while (per > 0 && at >= per) { at -= per; ++h; }
-  for (int it = hg - HG, turn = -HG; turn < total; turn += HG, it += HG, stage ^= kStage) {       // (every group as often: the barrier is everybody's)
+  auto fetch = [&](int stage) {
+    const unsigned t = lds + stage;
+    const int hd = kvh * group + h, r0 = first + at * BQ;
+    const long long ho = (long long)hd * a.dim * (int)sizeof(T);
+    rq.template fetch<kIssue>(qb + ho, r0, BQ, kg * kIssue, t, lane);
+    rd.template fetch<kIssue>(db + ho, r0, BQ, kg * kIssue, t + kTile, lane);
+    if (kg == 0) {                                           // delta, then lse of the tile's rows: four bytes a lane
+      const float* x = ga.delta + (g ? plane : 0) + (long long)hd * a.rows_q + qs + r0 + l31;
+      seq_dma4(r0 + l31 < nq ? (const void*)x : a.zero, t + 2 * kTile);
+    }
+    at += HG;
+    while (at >= per) { at -= per; ++h; }
+    return r0;
+  };
+  auto sees = [&](int row) { return !a.causal || row + 31 + ahead >= kw; };    // does any row of the tile see the wave's keys?
+  int r0 = 0, stage = 0;                                   // the first turn only fetches
+  for (int turn = -HG; turn < total; turn += HG, stage ^= kStage) {          // (every group as often: the barrier is everybody's)
+    const int it = turn + hg, row = r0;
     seq_dma_wait();
     if (KG > 1) __syncthreads();
-    const int row = r0;
-    if (it + HG < total) {
-      const unsigned t = lds + (stage ^ kStage);
-      const int hd = kvh * group + h;
-      const long long ho = (long long)hd * a.dim * (int)sizeof(T);
-      r0 = first + at * BQ;
-      rq.template fetch<kIssue>(qb + ho, r0, BQ, kg * kIssue, t, lane);
-      rd.template fetch<kIssue>(db + ho, r0, BQ, kg * kIssue, t + kTile, lane);
-      if (kg == 0) {                                         // delta, then lse of the tile's rows: four bytes a lane
-        const float* x = ga.delta + (g ? plane : 0) + (long long)hd * a.rows_q + qs + r0 + l31;
-        seq_dma4(r0 + l31 < nq ? (const void*)x : a.zero, t + 2 * kTile);
-      }
-      at += HG;
-      while (at >= per) { at -= per; ++h; }
-    }
-    if (turn < 0 || it >= total || (a.causal && row + 31 + ahead < kw)) continue;        // (or none of these rows sees the wave's keys)
-    const char *tq = base + stage, *td = tq + kTile;
-    const float *delta = reinterpret_cast<const float*>(td + kTile), *lse2 = delta + BQ;
-    {
-      f32x16 s, p;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
-#pragma unroll
-      for (int t = 0; t < DP / 16; ++t) {
-        s = seq_mma(seq_row<T, DP>(tq, l31, 2 * t + g), kf[t], s);
-        p = seq_mma(seq_row<T, DP>(td, l31, 2 * t + g), vf[t], p);
-      }
-      const bool masked = a.causal && row + ahead < kw + 31;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const sq_f4 ls = *reinterpret_cast<const sq_f4*>(lse2 + 8 * q + 4 * g), de = *reinterpret_cast<const sq_f4*>(delta + 8 * q + 4 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * q + e;
-          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[e])), y = x * (p[i] - de[e]);
-          if (masked) { const bool ok = key <= row + 8 * q + 4 * g + e + ahead; x = ok ? x : 0.f; y = ok ? y : 0.f; }
-          s[i] = x; p[i] = y;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const v8 pf = seq_pack<T>(s, t), sf = seq_pack<T>(p, t);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = seq_mma(seq_col<T, DP>(td, 16 * t, d, lane), pf, dv[d]);
-          dk[d] = seq_mma(seq_col<T, DP>(tq, 16 * t, d, lane), sf, dk[d]);
-        }
-      }
-    }
+    if (it + HG < total) r0 = fetch(stage ^ kStage);
+    if (turn < 0 || it >= total || !sees(row)) continue;
+    products(lds + stage);
+    weights(lds + stage);
+    if (a.causal && row + ahead < kw + 31) masks(row);
+    sums(lds + stage);
   }
   if (HG > 1) {                                              // the row groups' sums, in their order: dK, then dV through the same buffer
     constexpr int N = (DP / 32) * 16;
@@ -329,7 +367,7 @@ template <typename T, int DP, int RG, int KS> hipError_t grad_q(const SeqGradArg
 }
 template <typename T, int DP, int KG, int HG> hipError_t grad_kv(const SeqGradArgs& a, hipStream_t s) {
   static int done[kMaxDevices];
-  constexpr int tiles_lds = HG * 2 * (2 * 32 * SeqTile<T, DP>::kRow + 256), join = (HG - 1) * KG * (DP / 32) * 16 * 256, lds = tiles_lds > join ? tiles_lds : join;
+  constexpr int tiles_lds = HG * 2 * (2 * 32 * SeqTile<T, DP>::kRow + (SeqTile<T, DP>::kRow > 256 ? 512 : 256)), join = (HG - 1) * KG * (DP / 32) * 16 * 256, lds = tiles_lds > join ? tiles_lds : join;
   static_assert(lds <= 160 * 1024, "LDS");
   opt_in_dynamic_lds((const void*)seq_dkv_kernel<T, DP, KG, HG>, lds, done);
   const SeqArgs& f = a.f;

@@ -24,7 +24,7 @@ constexpr int kMaxSplits = 64;
 template <typename T, int DP, bool PAGED, int N>
 struct KeySource {
   typedef SeqTile<T, DP> L;
-  static constexpr int kRowsOf = SeqLanes<T, DP>::kRowsOf, kPeriod = SeqLanes<T, DP>::kPeriod;
+  static constexpr int kRowsOf = SeqLanes<T, DP>::kRowsOf;
   const char *k, *v; long long ldk, ldv;                     // bytes from a row to the next (paged: of a page)
   const int32_t* table; int last, shift, pages, kv_heads, head, dim, n; const void* zero;
   bool plain;                                                // whole tiles may go by scalar addresses
@@ -56,11 +56,12 @@ struct KeySource {
           pk = k + row * ldk; pv = v + row * ldv;
         }
         if (!there) { pk = pv = (const char*)zero; }
-        seq_dma16(pk, there ? wk.at[i % kPeriod] : 0u, tk + (first + i) * 1024);
-        seq_dma16(pv, there ? (PAGED ? wk : wv).at[i % kPeriod] : 0u, tv + (first + i) * 1024);
+        seq_dma16(pk, there ? wk.at(i) : 0u, tk + (first + i) * 1024);
+        seq_dma16(pv, there ? (PAGED ? wk : wv).at(i) : 0u, tv + (first + i) * 1024);
       }
       return;
     }
+    asm volatile("" : "+v"(lane));                           // (opaque: or what follows from it is kept in registers all the way)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = (first + i) * kRowsOf + lane / L::kChunks, c = (lane % L::kChunks) ^ L::turn(r), row = k0 + r;
@@ -90,10 +91,11 @@ struct Fwd {
   static constexpr int BN = RG == 4 ? 64 : 32, NJ = BN / 32, BM = 32 * RG;
   static constexpr int kTile = BN * L::kRow;                 // bytes of one K or V tile
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kLds = 2 * KS * kStage;               // a tile that is read and one on its way; more of them cost more in workgroups a unit than they hide (16 ragged f16: 20 -> 27 us)
+  static constexpr int kLds = 2 * KS * kStage + (3 * DP + 1) * 4;               // a tile that is read and one on its way; more of them cost more in workgroups a unit than they hide (16 ragged f16: 20 -> 27 us)
   static constexpr int kIssue = kTile / 1024 / RG;           // transfers of a wave for one tile of K (as many for V)
   static constexpr int kRegs = (DP / 32) * 16;               // accumulators of a lane
   static constexpr int kJoin = (KS - 1) * RG * (kRegs + 2) * 256;
+  static_assert(kJoin <= 2 * KS * kStage, "the join lies where the tiles were");
 };
 
 // The pieces of a row's keys joined by one wave, lanes along the channels
@@ -138,12 +140,12 @@ __device__ __forceinline__ void join_row(const SeqArgs& a, long long pr, long lo
 }
 
 template <typename T, int DP, bool PAGED, int RG, int KS>
-__global__ void __launch_bounds__(64 * RG * KS, (sizeof(T) == 2 && RG == 4) ? 2 : 1)
+__global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1)
 seq_fwd_kernel(const SeqArgs a, const int tiles) {
   typedef Fwd<T, DP, RG, KS> F;
   typedef SeqTile<T, DP> L;
   typedef typename F::v8 v8;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(512))) char smem[];         // (SeqReads: tiles start at multiples of their row)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG;
   const int l31 = lane & 31, g = lane >> 5;
 
@@ -192,7 +194,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
   } else {
     src.k = (const char*)a.k + (kstart * a.ldk + (long long)kvh * a.dim) * es; src.v = (const char*)a.v + (kstart * a.ldv + (long long)kvh * a.dim) * es;
     src.ldk = a.ldk * es; src.ldv = a.ldv * es;
-    src.plain = a.dim == DP && a.ldk < (1 << 24) && a.ldv < (1 << 24);         // (a lane's offset in 32 bits)
+    src.plain = a.dim == DP && a.ldk < (1 << 24) && a.ldv < (1 << 24) && !(src.ldk % L::kRow) && !(src.ldv % L::kRow);         // (SeqLanes; a lane's offset in 32 bits)
   }
   src.kv_heads = a.kv_heads; src.head = kvh; src.dim = a.dim; src.n = nk; src.zero = a.zero;
   src.wk.set((unsigned)src.ldk, lane, rg * F::kIssue);
@@ -217,13 +219,16 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
   constexpr int step = F::BN * KS;
   // ---- one tile: the logits of its keys, their weights, their share of the result -----------------------------------------------------
   f32x16 s[F::NJ];
-  auto logits = [&](const char* tk) {
+  SeqReads<T, DP> reads;
+  reads.set(lane);
+  auto logits = [&](unsigned tk) {
+    const unsigned at = seq_at(tk, reads.row);
 #pragma unroll
     for (int j = 0; j < F::NJ; ++j) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
 #pragma unroll
-      for (int t = 0; t < DP / 16; ++t) s[j] = seq_mma(seq_row<T, DP>(tk, 32 * j + l31, 2 * t + g), qf[t], s[j]);
+      for (int t = 0; t < DP / 16; ++t) s[j] = seq_mma(seq_row<T, DP>(at, 32 * j, t), qf[t], s[j]);
     }
   };
   auto weights = [&](int k0) {
@@ -255,20 +260,37 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) { s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc)); l += s[j][i]; }
   };
-  auto result = [&](const char* tv) {
+  auto result = [&](unsigned tv) {
+    const unsigned at = seq_at(tv, reads.col);
 #pragma unroll
     for (int j = 0; j < F::NJ; ++j)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const v8 p = seq_pack<T>(s[j], t);
+        if constexpr (sizeof(T) == 2 && (PAGED ? RG < 4 : RG == 1)) {      // (memory or latency bounds these: the second half of the weights is free)
+          v8 rest;
+          const v8 p = seq_pack<T>(s[j], t, rest);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) o[d] = seq_mma(seq_col<T, DP>(tv, 32 * j + 16 * t, d, lane), p, o[d]);
+          for (int d = 0; d < DP / 32; ++d) {
+            const v8 v = seq_col<T, DP>(at, 32 * j + 16 * t, d);
+            o[d] = seq_mma(v, p, o[d]);
+            o[d] = seq_mma(v, rest, o[d]);
+          }
+        } else {
+          const v8 p = seq_pack<T>(s[j], t);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) o[d] = seq_mma(seq_col<T, DP>(at, 32 * j + 16 * t, d), p, o[d]);
+        }
       }
   };
   const int mine = rg * F::kIssue;                           // this wave's first transfer of a tile
   // The first turn of the loop only fetches (one place in the code for it: short launches wait for their instructions, too).  Key groups go
   // through the loop equally often: its barrier is everybody's.
   seq_settle(qf);
+  int *what = reinterpret_cast<int*>(smem + 2 * KS * F::kStage), *flag = what + 3 * DP;         // seq_apart's, and the last tiles that needed it
+  for (int i = threadIdx.x; i < 3 * DP; i += 64 * RG * KS) what[i] = 0x7fffffff;
+  if (threadIdx.x == 0) *flag = -1;
+  if (RG == 1) __syncthreads();
+  const int all = seen(r0);                                  // what the workgroup's first row sees
   int stage = 0, k0 = k_begin + (kg - KS) * F::BN;
   src.look(k0 + step, mine);
   for (int kt = k_begin - step; kt < k_end; kt += step, k0 += step, stage ^= F::kStage) {
@@ -279,16 +301,28 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
       src.fetch(k0 + step, F::BN, mine, t, t + F::kTile, lane);
       src.look(k0 + 2 * step, mine);
     }
-    if (kt < k_begin || k0 >= k_end || k0 >= wsome) continue;
-    const char* tk = base + stage;
-    logits(tk);
+    if (kt < k_begin) continue;
+    // Where the diagonal runs through the tiles -- keys that are there and that some row does not see --: is any value in them not finite?
+    if (kt + step > all && all < nk) {
+      int me = rg * 64 + lane;                               // (an opaque copy: or the addresses below are kept in registers all the way)
+      asm volatile("" : "+v"(me));
+      if (k0 < k_end && seq_tainted<T, DP, F::BN>(base + stage + F::kTile, me, 64 * RG) && lane == 0) *flag = kt;
+      __syncthreads();
+      if (*flag == kt) {
+        if (k0 < k_end) seq_apart<T, DP, F::BN>(base + stage + F::kTile, what, k0, me, 64 * RG);
+        __syncthreads();
+      }
+    }
+    if (k0 >= k_end || k0 >= wsome) continue;
+    logits(lds + stage);
     weights(k0);
-    result(tk + F::kTile);
+    result(lds + stage + F::kTile);
   }
   l = seq_pair_sum(l);
 
+  __syncthreads();
+  const bool apart = *flag >= 0;                             // (in front of the join, which uses the tiles' place)
   if (KS > 1) {                                              // the key groups' parts of the same rows: the first group collects them
-    __syncthreads();
     float* x = reinterpret_cast<float*>(smem) + lane;        // [KS - 1][RG][registers, m, l][64]
     constexpr int N = F::kRegs;
     if (kg > 0) {
@@ -310,6 +344,25 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * f1 + y[(16 * d + i) * 64] * f2;
     }
+  }
+  if (apart) {
+    int half = g;
+    asm volatile("" : "+v"(half));
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        typedef int i4 __attribute__((ext_vector_type(4)));
+        const i4* w = reinterpret_cast<const i4*>(what + 32 * d + 8 * (i >> 2) + 4 * half);
+        const i4 up = w[0], down = w[DP / 4], none = w[DP / 2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (up[e] < limit) o[d][i + e] += __builtin_inff();
+          if (down[e] < limit) o[d][i + e] -= __builtin_inff();
+          if (none[e] < limit) o[d][i + e] = __builtin_nanf("");
+        }
+        asm volatile("" ::: "memory");                       // (four channels at a time: this is rare, registers are not)
+      }
   }
   if (PAGED && a.splits > 1) {
     const long long n = (long long)a.rows_q * a.heads;
