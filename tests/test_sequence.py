@@ -276,6 +276,8 @@ PACKED = [
     ([3, 260], [260, 3], 2, 2, 72, False),
     ([0, 0, 9], [4, 0, 9], 2, 1, 64, True),                       # keys that no row sees
     ([300], None, 1, 1, 128, True),
+    ([530], None, 2, 1, 64, True),                                # rows enough for the launches of long sequences
+    ([400, 633], [633, 400], 4, 2, 128, True),
 ]
 IDS = ["-".join([str(i)]) for i in range(len(PACKED))]
 

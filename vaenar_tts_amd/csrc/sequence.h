@@ -256,7 +256,7 @@ __device__ __forceinline__ int seq_scalar(const int32_t* p) {
 // other[b], x1 = other[b + two], fetched along with the starts.  Where the launch has more workgroups than the chip
 // holds at once, up to 64 sequences are gone through from the longest (rows, or rows + x0 where x0 counts keys in front of them: `two` 0) to
 // the shortest: it ends with its short tasks (eight chunks of up to 512 rows over up to 6000 keys: 223 -> 187 us; about 1 us of a small launch).
-struct SeqWhere { int b, tile, start, n, x0, x1; };
+struct SeqWhere { int b, rank, tile, start, n, x0, x1; };         // rank: of the sequence in the order of the tasks
 __device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total, int mult, int rows, int index, const int32_t* other, int two, SeqWhere& w) {
   const int lane = threadIdx.x & 63;
   int before = 0;
@@ -285,6 +285,7 @@ __device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total
     const unsigned long long m = __builtin_amdgcn_ballot_w64(index < before + x);
     if (m) {
       const int src = __builtin_ctzll(m);
+      w.rank = b0 + src;
       w.tile = index - before - __builtin_amdgcn_readlane(x - t, src);
       w.b = __builtin_amdgcn_readlane(b, src); w.start = __builtin_amdgcn_readlane(s, src); w.n = __builtin_amdgcn_readlane(n, src);
       w.x0 = __builtin_amdgcn_readlane(x0, src); w.x1 = __builtin_amdgcn_readlane(x1, src);

@@ -86,11 +86,8 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
     delta = seq_pair_sum(delta);
   }
   float lse2 = 0.f;
-  if (live) {
-    const long long at = (long long)head * a.rows_q + token, plane = (long long)a.heads * a.rows_q;
-    lse2 = a.lse[at] * kLog2e;
-    if (g == 0 && kg == 0) { ga.delta[at] = delta; ga.delta[plane + at] = lse2; }
-  }
+  const long long place = (long long)head * a.rows_q + token;
+  if (live) lse2 = a.lse[place] * kLog2e;
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -104,10 +101,47 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
   Rows<T, DP> rk, rv;
   rk.set(a.ldk, nk, a.dim, a.zero, lane, rg * kIssue); rv.set(a.ldv, nk, a.dim, a.zero, lane, rg * kIssue);
   seq_settle(qf); seq_settle(df);
+  auto products = [&](unsigned tk, int j, f32x16& s, f32x16& p) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      s = seq_mma(seq_row<T, DP>(tk, 32 * j, t), qf[t], s);
+      p = seq_mma(seq_row<T, DP>(tk, BN + 32 * j, t), df[t], p);           // (V lies behind K)
+    }
+  };
+  // The rounding of `out` reaches dS through delta, and where few keys share a row's weight nothing averages it away (rows of up to 8 keys: dQ 1.7
+  // times as far from 64 bits as a plain form's).  Up to 64 keys: delta = sum_j P dP instead, in a turn of its own.
+  if (sizeof(T) == 2 && nk <= 64) {
+    float sum = 0.f;
+    for (int kt = -BN, stage = 0; kt < some; kt += BN, stage ^= kStage) {
+      seq_dma_wait();
+      __syncthreads();
+      if (kt + BN < some) {
+        const unsigned t = lds + (stage ^ kStage);
+        rk.template fetch<kIssue>(kb, kt + BN, BN, rg * kIssue, t, lane);
+        rv.template fetch<kIssue>(vb, kt + BN, BN, rg * kIssue, t + kTile, lane);
+      }
+      if (kt < 0 || kt >= wsome) continue;
+      const unsigned tk = seq_at(lds + stage, reads.row);
+#pragma unroll
+      for (int j = 0; j < BN / 32; ++j) {
+        f32x16 s, p;
+        products(tk, j, s, p);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2)) * p[i];
+          sum += kt + 32 * j + 8 * (i >> 2) + 4 * g + (i & 3) < limit ? x : 0.f;
+        }
+      }
+    }
+    delta = seq_pair_sum(sum);
+  }
+  if (live && g == 0 && kg == 0) { ga.delta[place] = delta; ga.delta[(long long)a.heads * a.rows_q + place] = lse2; }
   int k0 = (kg - KS) * BN, stage = 0;                        // (the first turn only fetches)
   for (int kt = -step; kt < some; kt += step, k0 += step, stage ^= kStage) {
     seq_dma_wait();
-    if (RG > 1) __syncthreads();
+    __syncthreads();
     if (k0 + step < some) {
       const unsigned t = lds + (stage ^ kStage);
       rk.template fetch<kIssue>(kb, k0 + step, BN, rg * kIssue, t, lane);
@@ -119,13 +153,7 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
 #pragma unroll
     for (int j = 0; j < BN / 32; ++j) {
       f32x16 s, p;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { s[i] = 0.f; p[i] = 0.f; }
-#pragma unroll
-      for (int t = 0; t < DP / 16; ++t) {
-        s = seq_mma(seq_row<T, DP>(tk, 32 * j, t), qf[t], s);
-        p = seq_mma(seq_row<T, DP>(tk, BN + 32 * j, t), df[t], p);         // (V lies behind K)
-      }
+      products(tk, j, s, p);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2)) * (p[i] - delta);
       if (masked) {
@@ -187,7 +215,7 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
 // through LDS in tiles of 32.  HG row groups of waves take the tiles in turn (each with buffers of its own) and their sums are joined at the
 // end: a sequence's first keys are seen by all of its rows in every head, one wave for them would outlast the rest of the launch.
 template <typename T, int DP, int KG, int HG>
-__global__ void __launch_bounds__(64 * KG * HG, sizeof(T) == 2 ? 2 : 1) seq_dkv_kernel(const SeqGradArgs ga, const int tiles) {
+__global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128 ? 2 : 1) seq_dkv_kernel(const SeqGradArgs ga, const int tiles) {
   typedef SeqTile<T, DP> L;
   typedef typename SeqVec<T>::v8 v8;
   const SeqArgs& a = ga.f;
@@ -202,7 +230,9 @@ __global__ void __launch_bounds__(64 * KG * HG, sizeof(T) == 2 ? 2 : 1) seq_dkv_
   int qs, nq;
   seq_clamp(w.x0, w.x1, a.rows_q, qs, nq);
   const int nk = w.n, ahead = nk - nq;
-  const int k0 = w.tile * BK, kw = k0 + 32 * kg, key = kw + l31;
+  // The first keys of a sequence are seen by most rows.  Two workgroups share a compute unit, the second of them about a sequence further in
+  // the tasks' order: every other sequence goes from its light end, so that a heavy one meets a light one.
+  const int k0 = (w.rank & 1 ? (nk + BK - 1) / BK - 1 - w.tile : w.tile) * BK, kw = k0 + 32 * kg, key = kw + l31;
   const bool live = key < nk;
   v8 kf[DP / 16], vf[DP / 16];
   {
@@ -385,6 +415,10 @@ template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, int cus, hip
   const long long wgs = ((long long)f.rows_q / 128 + (f.batch < f.rows_q ? f.batch : f.rows_q)) * f.heads;
   if (f.rows_q > 0) e = wgs >= 2LL * cus ? grad_q<T, DP, 4, 1>(a, s) : grad_q<T, DP, 2, 2>(a, s);
   if (e != hipSuccess || f.rows_k == 0) return e;
+  // Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 208 -> 174 us
+  // for dK and dV), two of them and twice the workgroups a unit where they pass few (the f32 case 78 -> 65); rows of 512 bytes leave room for two
+  const long long turns = (long long)f.rows_q / f.batch * (f.heads / f.kv_heads) / 32;
+  if (sizeof(T) * DP <= 256 && turns >= 32) return grad_kv<T, DP, 2, (sizeof(T) * DP > 256 ? 2 : 4)>(a, s);
   return grad_kv<T, DP, 2, 2>(a, s);
 }
 template <typename T> hipError_t grad(const SeqGradArgs& a, int cus, hipStream_t s) { return a.f.dim <= 64 ? grad<T, 64>(a, cus, s) : grad<T, 128>(a, cus, s); }
