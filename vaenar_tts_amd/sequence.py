@@ -15,6 +15,7 @@ import numpy as np
 from ._lib import (VnrError, vnr_kv_append_desc, vnr_kv_cache, vnr_packed_attention_desc, vnr_packed_attention_grad,
                    vnr_paged_attention_desc)
 
+_I32, _F32 = np.dtype(np.int32), np.dtype(np.float32)
 _CODES = {np.dtype(np.float32): 0, np.dtype(np.float16): 1, np.dtype(np.uint16): 2}
 
 
@@ -32,17 +33,18 @@ def from_bf16(x):
 
 
 def _code(who, first, *others):
-    code = _CODES.get(first.dtype)
+    kind = first.dtype
+    code = _CODES.get(kind)
     if code is None:
         raise VnrError("%s: float32, float16 or uint16 (bfloat16 bits) arrays, not %s" % (who, first.dtype))
     for a in others:
-        if a is not None and a.dtype != first.dtype:
+        if a is not None and a.dtype is not kind and a.dtype != kind:
             raise VnrError("%s: arrays of one type: %s and %s" % (who, first.dtype, a.dtype))
     return code
 
 
 def _ints(who, name, a, shape):
-    if a.dtype != np.int32 or a.shape != shape:
+    if (a.dtype is not _I32 and a.dtype != _I32) or a.shape != shape:
         raise VnrError("%s: %s must be int32 %s, not %s %s" % (who, name, shape, a.dtype, a.shape))
 
 
@@ -52,7 +54,7 @@ def _shape(who, name, a, shape):
 
 
 def _floats(who, name, a, shape):
-    if a.dtype != np.float32 or a.shape != shape:
+    if (a.dtype is not _F32 and a.dtype != _F32) or a.shape != shape:
         raise VnrError("%s: %s must be float32 %s, not %s %s" % (who, name, shape, a.dtype, a.shape))
 
 
@@ -123,9 +125,9 @@ class PagedCache:
         _shape(who, "v", v, k.shape)
         self.engine, self.k, self.v = engine, k, v
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        self._code = _code(who, k, v)
+        self._kind, self._row = k.dtype, (self.kv_heads, self.head_dim)
         # fixed for the cache's life: the calls that a range trip makes the engine issue again point to it
-        self._desc = vnr_kv_cache(self._code, self.kv_heads, self.head_dim, self.pages, self.page_size, k.ptr, v.ptr)
+        self._desc = vnr_kv_cache(_code(who, k, v), self.kv_heads, self.head_dim, self.pages, self.page_size, k.ptr, v.ptr)
         self._ref = C.byref(self._desc)
 
     @classmethod
@@ -135,11 +137,14 @@ class PagedCache:
 
     def _batch(self, who, cu, context, table):
         batch = cu.shape[0] - 1
-        _ints(who, "cu", cu, (batch + 1,))
-        _ints(who, "context", context, (batch,))
-        if len(table.shape) != 2:
-            raise VnrError("%s: table must be [batch, table_width]" % who)
-        _ints(who, "table", table, (batch, table.shape[1]))
+        # (one look where all is well: a decoding step is a few microseconds long)
+        if not (cu.dtype is _I32 and context.dtype is _I32 and table.dtype is _I32 and context.shape == (batch,) and len(cu.shape) == 1
+                and len(table.shape) == 2 and table.shape[0] == batch):
+            _ints(who, "cu", cu, (batch + 1,))
+            _ints(who, "context", context, (batch,))
+            if len(table.shape) != 2:
+                raise VnrError("%s: table must be [batch, table_width]" % who)
+            _ints(who, "table", table, (batch, table.shape[1]))
         return batch
 
     def append(self, k, v, cu, context, table, rotation=None, q=None, q_out=None, interleaved=False, ldk=None, ldv=None, ldq=None, ldqo=None):
@@ -149,8 +154,9 @@ class PagedCache:
         who = "PagedCache.append"
         batch = self._batch(who, cu, context, table)
         rows = k.shape[0]
-        _shape(who, "k", k, (rows, self.kv_heads, self.head_dim))
-        _shape(who, "v", v, k.shape)
+        if not (k.shape == v.shape and k.shape[1:] == self._row):
+            _shape(who, "k", k, (rows,) + self._row)
+            _shape(who, "v", v, k.shape)
         heads = 0
         if q is not None:
             heads = q.shape[1]
@@ -160,8 +166,9 @@ class PagedCache:
             _shape(who, "q_out", q_out, q.shape)
         elif q_out is not None:
             raise VnrError("%s: q_out without q" % who)
-        _code(who, self.k, k, v, q, q_out)
-        if rotation is not None and (rotation.dtype != np.float32 or len(rotation.shape) != 2):
+        if not (k.dtype is v.dtype is self._kind and (q is None or q.dtype is q_out.dtype is self._kind)):
+            _code(who, self.k, k, v, q, q_out)
+        if rotation is not None and (rotation.dtype != _F32 or len(rotation.shape) != 2):
             raise VnrError("%s: rotation must be float32 [positions, rot_dim]" % who)
         rot = (None, 0, 0) if rotation is None else (rotation.ptr,) + rotation.shape
         wk, wq = self.kv_heads * self.head_dim, heads * self.head_dim
@@ -183,7 +190,8 @@ class PagedCache:
         if out is None:
             out = self.engine.empty(q.shape, q.dtype)
         _shape(who, "out", out, q.shape)
-        _code(who, self.k, q, out)
+        if not q.dtype is out.dtype is self._kind:
+            _code(who, self.k, q, out)
         if lse is not None:
             _floats(who, "lse", lse, (heads, rows))
         wq = heads * self.head_dim
