@@ -108,6 +108,27 @@ __device__ __forceinline__ unsigned seq_at(unsigned tile, unsigned lane) {
   return x;
 }
 template <typename V> __device__ __forceinline__ V seq_ds(unsigned at) { return *(const __attribute__((address_space(3))) V*)at; }
+// A run of N products whose operands come from LDS, two at a time: the next two reads are issued in front of these two products.  Left alone the
+// compiler saves registers it need not save -- read, wait for LDS, multiply, read ... -- and every product waits out a read: 4 prompts of up to 4096
+// rows (32 heads of 128, bf16) 435 us so, 417 us here; four at a time 421.  (0x406: arithmetic and scalar work may still cross.)
+template <typename T, int N, typename Load, typename Mul> __device__ __forceinline__ void seq_run(Load&& load, Mul&& mul) {
+  constexpr int B = 2;
+  static_assert(N % B == 0, "whole batches");
+  typename SeqVec<T>::v8 x[2][B];
+#pragma unroll
+  for (int i = 0; i < B; ++i) x[0][i] = load(i);
+#pragma unroll
+  for (int b = 0; b < N / B; ++b) {
+    if (b + 1 < N / B) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) x[(b + 1) & 1][i] = load((b + 1) * B + i);
+    }
+    __builtin_amdgcn_sched_barrier(0x406);
+#pragma unroll
+    for (int i = 0; i < B; ++i) mul(b * B + i, x[b & 1][i]);
+    __builtin_amdgcn_sched_barrier(0x406);
+  }
+}
 // at: seq_at(tile, reads.row); rows r0 .. r0 + 31 of the tile
 template <typename T, int DP> __device__ __forceinline__ typename SeqVec<T>::v8 seq_row(unsigned at, int r0, int t) {
   typedef SeqTile<T, DP> L;

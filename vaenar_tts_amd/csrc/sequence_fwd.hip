@@ -224,12 +224,11 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
   auto logits = [&](unsigned tk) {
     const unsigned at = seq_at(tk, reads.row);
 #pragma unroll
-    for (int j = 0; j < F::NJ; ++j) {
+    for (int j = 0; j < F::NJ; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
-#pragma unroll
-      for (int t = 0; t < DP / 16; ++t) s[j] = seq_mma(seq_row<T, DP>(at, 32 * j, t), qf[t], s[j]);
-    }
+    constexpr int n = DP / 16;
+    seq_run<T, F::NJ * n>([&](int i) { return seq_row<T, DP>(at, 32 * (i / n), i % n); }, [&](int i, const v8& k) { s[i / n] = seq_mma(k, qf[i % n], s[i / n]); });
   };
   auto weights = [&](int k0) {
     if (k0 + F::BN > wall) {                                 // (the wave's first row does not see the whole tile)
@@ -262,25 +261,17 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
   };
   auto result = [&](unsigned tv) {
     const unsigned at = seq_at(tv, reads.col);
-#pragma unroll
-    for (int j = 0; j < F::NJ; ++j)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if constexpr (sizeof(T) == 2 && (PAGED ? RG < 4 : RG == 1)) {      // (memory or latency bounds these: the second half of the weights is free)
-          v8 rest;
-          const v8 p = seq_pack<T>(s[j], t, rest);
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) {
-            const v8 v = seq_col<T, DP>(at, 32 * j + 16 * t, d);
-            o[d] = seq_mma(v, p, o[d]);
-            o[d] = seq_mma(v, rest, o[d]);
-          }
-        } else {
-          const v8 p = seq_pack<T>(s[j], t);
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) o[d] = seq_mma(seq_col<T, DP>(at, 32 * j + 16 * t, d), p, o[d]);
-        }
-      }
+    constexpr int n = DP / 32;
+    constexpr bool fine = sizeof(T) == 2 && (PAGED ? RG < 4 : RG == 1);      // (memory or latency bounds these: the second half of the weights is free)
+    v8 p, rest;
+    seq_run<T, F::NJ * 2 * n>([&](int i) { return seq_col<T, DP>(at, 16 * (i / n), i % n); },
+                              [&](int i, const v8& v) {
+                                if (i % n == 0) {
+                                  if constexpr (fine) p = seq_pack<T>(s[i / n / 2], i / n % 2, rest); else p = seq_pack<T>(s[i / n / 2], i / n % 2);
+                                }
+                                o[i % n] = seq_mma(v, p, o[i % n]);
+                                if constexpr (fine) o[i % n] = seq_mma(v, rest, o[i % n]);
+                              });
   };
   const int mine = rg * F::kIssue;                           // this wave's first transfer of a tile
   // The first turn of the loop only fetches (one place in the code for it: short launches wait for their instructions, too).  Key groups go
