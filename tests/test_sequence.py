@@ -349,6 +349,28 @@ def test_packed_attention_on_column_blocks(eng, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_with_one_key_add_exactly_nothing_to_dq_and_dk(eng, dim, kind):
+    """Their weight is 1 whatever the logit: no rounding of delta may be left over, not even where all of dQ and dK is made of such rows."""
+    r = np.random.default_rng(dim)
+
+    def gradients(lq, lk, causal):
+        cu_q, cu_k = starts(lq), starts(lk)
+        q, k, v, do = (eng.to_device(normal(r, kind, n, h, dim)) for n, h in ((cu_q[-1], 8), (cu_k[-1], 2), (cu_k[-1], 2), (cu_q[-1], 8)))
+        cq, ck = eng.to_device(cu_q), eng.to_device(cu_k)
+        out, lse = sequence.packed_attention(eng, q, k, v, cq, ck, causal)
+        return [value(x.numpy()) for x in sequence.packed_attention_grad(eng, do, q, k, v, out, lse, cq, ck, causal)]
+
+    for lq, lk, causal in (([1] * 7, [1] * 7, True), ([1] * 3, [1] * 3, False), ([40, 1, 300], [1, 1, 1], False), ([40, 300], [1, 1], True)):
+        dq, dk, dv = gradients(lq, lk, causal)
+        assert (dq == 0).all() and (dk == 0).all() and (dv != 0).any()
+    # of longer sequences the first row that sees a key: row 0, and row 20 of the one with more rows than keys
+    dq, dk, dv = gradients([50, 300, 120], [50, 300, 100], True)
+    assert (dq[[0, 50, 350 + 20]] == 0).all() and (dq[[1, 51, 350 + 21]] != 0).any()
+
+
+@pytest.mark.gpu
 def test_packed_gradient_has_the_same_bits_every_time(eng):
     r = np.random.default_rng(4)
     cu = starts([200, 90, 333])

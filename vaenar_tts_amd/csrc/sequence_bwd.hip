@@ -201,13 +201,14 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
     }
   }
   if (!live) return;
+  const float out = limit == 1 ? 0.f : a.scale;              // one key: its weight is 1 whatever the logit, dQ is exactly nothing (not a rounding of delta)
   T* dq = (T*)ga.dq + token * ga.lddq + (long long)head * a.dim;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int col = 32 * d + 8 * (i >> 2) + 4 * g;
-      if (col < a.dim) seq_store4<T>(dq + col, acc[d][i] * a.scale, acc[d][i + 1] * a.scale, acc[d][i + 2] * a.scale, acc[d][i + 3] * a.scale);
+      if (col < a.dim) seq_store4<T>(dq + col, acc[d][i] * out, acc[d][i + 1] * out, acc[d][i + 2] * out, acc[d][i + 3] * out);
     }
 }
 
@@ -295,6 +296,10 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
       const bool ok = key <= row + 8 * (i >> 2) + 4 * g + (i & 3) + ahead;
       s[i] = ok ? s[i] : 0.f; p[i] = ok ? p[i] : 0.f;
     }
+    if (row + ahead > 0) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)                             // (the row that sees key 0 alone: it adds exactly nothing to dK)
+      if (row + 8 * (i >> 2) + 4 * g + (i & 3) + ahead == 0) p[i] *= 0.f;
   };
   auto sums = [&](unsigned tile) {
     const unsigned at = seq_at(tile, reads.col);
@@ -370,6 +375,7 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
     if (hg > 0) return;
   }
   if (!live) return;
+  const float out = nk == 1 ? 0.f : a.scale;                 // (as in dQ)
   T *pk = (T*)ga.dk + (w.start + key) * ga.lddk + (long long)kvh * a.dim, *pv = (T*)ga.dv + (w.start + key) * ga.lddv + (long long)kvh * a.dim;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -377,7 +383,7 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
     for (int i = 0; i < 16; i += 4) {
       const int col = 32 * d + 8 * (i >> 2) + 4 * g;
       if (col < a.dim) {
-        seq_store4<T>(pk + col, dk[d][i] * a.scale, dk[d][i + 1] * a.scale, dk[d][i + 2] * a.scale, dk[d][i + 3] * a.scale);
+        seq_store4<T>(pk + col, dk[d][i] * out, dk[d][i + 1] * out, dk[d][i + 2] * out, dk[d][i + 3] * out);
         seq_store4<T>(pv + col, dv[d][i], dv[d][i + 1], dv[d][i + 2], dv[d][i + 3]);
       }
     }
