@@ -281,7 +281,9 @@ typedef struct vnr_packed_attention_grad {
 /* out = softmax(scale q k' + mask) v of every sequence (MultiHeadScaledProductAttention.call, modules/attention.py:224-246, without its
  * padding).  A row that sees no key: zeros, d_lse = -infinity. */
 int vnr_op_packed_attention(vnr_handle h, const vnr_packed_attention_desc *desc);
-/* Its gradient, from the forward's d_out and d_lse.  No atomics: the same bits every time.  Rows and keys that see nothing get zeros. */
+/* Its gradient, from the forward's d_out and d_lse.  No atomics: the same bits every time.  Rows and keys that see nothing get zeros, and a
+ * row that sees one key adds exactly nothing to dq and dk.  The exception to masked keys' silence: where q, k, v or dout of a sequence's own
+ * rows are not finite, gradients of that sequence may be NaN also in rows that do not see them (other sequences' are not touched by it). */
 int vnr_op_packed_attention_grad(vnr_handle h, const vnr_packed_attention_desc *desc, const vnr_packed_attention_grad *grad);
 
 /* Pools of pages, [pages][kv_heads][page_size][head_dim] each; position p of sequence b lives in page d_table[b][p / page_size].
@@ -295,7 +297,8 @@ int vnr_op_rotation_table(vnr_handle h, int positions, int rot_dim, double base,
 /* New keys and values of a batch into the cache: row d_cu[b] + i goes to position d_context[b] + i of sequence b.  The first rot_dim
  * channels of a key turn by their position on the way (channel c with c + rot_dim / 2, or with interleaved = 1 channel 2 c with 2 c + 1);
  * rot_dim = 0: no rotation.  With d_q the queries of the same rows turn too, into d_q_out (not in place).  A position behind the table's
- * end is dropped; so are K and V of one whose page is none of the pool's (a negative number, say). */
+ * end is dropped; so are K and V of one whose page is none of the pool's (a negative number, say).  Sequences may share the pages of a common
+ * beginning; a position that two rows of one call are written to holds either of them.  rows < 2^24. */
 typedef struct vnr_kv_append_desc {
   int32_t batch, heads, rows;              /* heads: of d_q */
   const int32_t *d_cu, *d_context, *d_table; int32_t table_width;      /* [batch + 1], [batch], [batch][table_width] */

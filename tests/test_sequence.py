@@ -231,6 +231,16 @@ def test_library_refusals_of_cache_calls():
         assert word in refused("vnr_op_paged_attention", K(**cache), P(**{**att, **bad})), bad
 
 
+def test_library_refusals_of_sizes_that_no_launch_holds():
+    assert "scale" in refused("vnr_op_packed_attention", packed_desc(scale=3e38))
+    assert "heads" in refused("vnr_op_packed_attention", packed_desc(heads=1 << 21, ldq=1 << 27, ldo=1 << 27))
+    cache = _lib.vnr_kv_cache(dtype=1, kv_heads=2, head_dim=64, pages=8, page_size=16, d_k=4096, d_v=4096)
+    assert "2^24" in refused("vnr_op_kv_append", cache, _lib.vnr_kv_append_desc(batch=1, rows=1 << 24, d_cu=64, d_context=64, d_table=64, table_width=3, d_k=4096, d_v=4096,
+                                                                               ldk=128, ldv=128))
+    lib = _lib.load()
+    assert lib.vnr_op_rotation_table(None, 1 << 30, 128, 1e4, C.c_void_p(4096)) == -1 and "2^31" in lib.vnr_last_error(None).decode()
+
+
 def test_sequence_structs_match_the_header_layout(tmp_path):
     import os
     import subprocess

@@ -397,7 +397,7 @@ template <typename T, int DP, int RG, int KS> hipError_t grad_q(const SeqGradArg
   const SeqArgs& f = a.f;
   const int tiles = f.rows_q / (32 * RG) + (f.batch < f.rows_q ? f.batch : f.rows_q);
   const long long grid = (long long)tiles * f.heads;
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (grid >= 1 << 24) return hipErrorInvalidValue;           // (2^32 threads)
   vnr_launch(seq_dq_kernel<T, DP, RG, KS>, dim3((unsigned)grid), dim3(64 * RG * KS), lds, s, a, tiles);
   return hipGetLastError();
 }
@@ -409,7 +409,7 @@ template <typename T, int DP, int KG, int HG> hipError_t grad_kv(const SeqGradAr
   const SeqArgs& f = a.f;
   const int tiles = f.rows_k / (32 * KG) + (f.batch < f.rows_k ? f.batch : f.rows_k);
   const long long grid = (long long)tiles * f.kv_heads;
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (grid >= (1LL << 32) / (64 * KG * HG)) return hipErrorInvalidValue;
   vnr_launch(seq_dkv_kernel<T, DP, KG, HG>, dim3((unsigned)grid), dim3(64 * KG * HG), lds, s, a, tiles);
   return hipGetLastError();
 }

@@ -98,6 +98,12 @@ struct Fwd {
   static_assert(kJoin <= 2 * KS * kStage, "the join lies where the tiles were");
 };
 
+// A row's bound in units of log2, rounded once and the same wherever it is used: weights of different tiles stay in proportion
+__device__ __forceinline__ float bound(float m, float c) {
+#pragma clang fp contract(off)
+  return m * c;
+}
+
 // The pieces of a row's keys joined by one wave, lanes along the channels
 template <typename T>
 __device__ __forceinline__ void join_row(const SeqArgs& a, long long pr, long long n, int token, int head, int lane) {
@@ -245,7 +251,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     mx = seq_pair_max(mx);
     if (__builtin_amdgcn_ballot_w64((mx - m) * c > kBound || (mx > m && m == -__builtin_inff()))) {
       const float m1 = fmaxf(m, mx);
-      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - m1) * c);
+      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound(m, c) - bound(m1, c));
       m = m1;
       l *= f;
 #pragma unroll
@@ -253,7 +259,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= f;
     }
-    const float mc = m == -__builtin_inff() ? 0.f : m * c;
+    const float mc = m == -__builtin_inff() ? 0.f : bound(m, c);
 #pragma unroll
     for (int j = 0; j < F::NJ; ++j)
 #pragma unroll
@@ -328,7 +334,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     for (int k = 0; kg == 0 && k < KS - 1; ++k) {
       const float* y = x + (k * RG + rg) * (N + 2) * 64;
       const float m2 = y[N * 64], l2 = y[(N + 1) * 64], m1 = fmaxf(m, m2);
-      const float f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - m1) * c), f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m2 - m1) * c);
+      const float mc = bound(m1, c), f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound(m, c) - mc), f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound(m2, c) - mc);
       m = m1; l = l * f1 + l2 * f2;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -359,7 +365,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     const long long n = (long long)a.rows_q * a.heads;
     if (live && kg == 0) {
       const long long pr = split * n + (long long)token * a.heads + head;
-      if (g == 0) { const sq_f2 x = {m == -__builtin_inff() ? m : m * c, l}; *reinterpret_cast<sq_f2*>(a.ml + 2 * pr) = x; }
+      if (g == 0) { const sq_f2 x = {m == -__builtin_inff() ? m : bound(m, c), l}; *reinterpret_cast<sq_f2*>(a.ml + 2 * pr) = x; }
       float* op = a.part + pr * a.dim;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -381,7 +387,8 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
       const int col = 32 * d + 8 * (i >> 2) + 4 * g;
       if (col < a.dim) seq_store4<T>(op + col, o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv, o[d][i + 3] * inv);
     }
-  if (a.lse && g == 0) a.lse[(long long)head * a.rows_q + token] = l != 0.f ? m * a.scale + __logf(l) : -__builtin_inff();
+  // the weights are relative to the ROUNDED bound; what its rounding left belongs to the sum
+  if (a.lse && g == 0) a.lse[(long long)head * a.rows_q + token] = l != 0.f ? m * a.scale + (__logf(l) - kLn2 * __builtin_fmaf(m, c, -bound(m, c))) : -__builtin_inff();
 }
 
 template <typename T>
@@ -407,7 +414,7 @@ hipError_t fwd(const SeqArgs& a, hipStream_t s) {
   opt_in_dynamic_lds((const void*)seq_fwd_kernel<T, DP, PAGED, RG, KS>, lds, done);
   const int mult = PAGED ? a.heads / a.kv_heads : 1, tiles = tiles_of(a, mult, F::BM);
   const long long grid = (long long)tiles * (PAGED ? (long long)a.kv_heads * a.splits : a.heads);
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (grid >= 1 << 24) return hipErrorInvalidValue;           // (2^32 threads)
   vnr_launch(seq_fwd_kernel<T, DP, PAGED, RG, KS>, dim3((unsigned)grid), dim3(64 * RG * KS), lds, s, a, tiles);
   return hipGetLastError();
 }
@@ -455,7 +462,7 @@ hipError_t launch_seq_fwd(const SeqArgs& a, const SeqPlan& p, hipStream_t s) {
 }
 hipError_t launch_seq_join(const SeqArgs& a, hipStream_t s) {
   const long long n = (long long)a.rows_q * a.heads, grid = (n + 3) / 4;
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (grid >= 1 << 24) return hipErrorInvalidValue;           // (2^32 threads)
   if (a.dtype == SEQ_F32) vnr_launch(seq_join_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, a);
   else if (a.dtype == SEQ_F16) vnr_launch(seq_join_kernel<_Float16>, dim3((unsigned)grid), dim3(256), 0, s, a);
   else vnr_launch(seq_join_kernel<sq_bf16>, dim3((unsigned)grid), dim3(256), 0, s, a);
