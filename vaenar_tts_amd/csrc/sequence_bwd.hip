@@ -1,9 +1,15 @@
 // Attention backward on packed sequences.  With P = exp(scale S - lse), dP = dO V', delta_i = sum_d dO_id O_id:
 //   dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS' Q,  dV = P' dO.
 // Two kernels, each the owner of what it writes (no atomics: the same bits every time, and the heads of a group are summed inside the
-// workgroup that owns their keys): seq_dq_kernel goes over the keys of its 128 query rows, seq_dkv_kernel over the query rows (of every head
-// of the group) of its 128 keys.  Both rebuild S and dP -- seven products instead of the five that one pass with atomics onto dQ would take.
-// P and dS are rounded to the operands' type for the products that read them; every sum is held in 32 bits.
+// workgroup that owns their keys): seq_dq_kernel goes over the keys of its query rows, seq_dkv_kernel over the query rows (of every head
+// of the group) of its keys.  Both rebuild S and dP -- seven products instead of the five that one pass with atomics onto dQ would take.
+// P is rounded once to the operands' type for dV (as dout is); what that rounding leaves of dS goes through a second product in 16-bit types --
+// the differences dP - delta cancel, and a rounding of what is left shows in dQ and dK (with it they are within 1.1 of the error of a plain
+// form in 32 bits whose results are rounded once, dV within 1.4).  Every sum is held in 32 bits.
+//
+// What bounds it: 4 sequences of up to 2048 rows, 32 heads over 8 of 128, bf16, causal: 256 us, 106 for dQ and 171 for dK and dV -- nine products
+// where the formulas have five, 0.79 PFLOP/s of them; a workgroup of dK and dV lasts as long as the rows that see its keys.  32 utterances of
+// up to 400 rows, 4 heads of 64, f32: 113 us (52 + 66), the 32-bit matrix instructions' rate and LDS reads of four bytes a lane.
 #include "sequence.h"
 
 namespace vnr {
@@ -293,13 +299,10 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
   auto masks = [&](int row) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const bool ok = key <= row + 8 * (i >> 2) + 4 * g + (i & 3) + ahead;
-      s[i] = ok ? s[i] : 0.f; p[i] = ok ? p[i] : 0.f;
+      const int sees = row + 8 * (i >> 2) + 4 * g + (i & 3) + ahead;
+      const float f = sees == 0 ? 0.f : p[i];                // (the row that sees key 0 alone adds exactly nothing to dK)
+      s[i] = key <= sees ? s[i] : 0.f; p[i] = key <= sees ? f : 0.f;
     }
-    if (row + ahead > 0) return;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)                             // (the row that sees key 0 alone: it adds exactly nothing to dK)
-      if (row + 8 * (i >> 2) + 4 * g + (i & 3) + ahead == 0) p[i] *= 0.f;
   };
   auto sums = [&](unsigned tile) {
     const unsigned at = seq_at(tile, reads.col);
@@ -417,12 +420,12 @@ template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, int cus, hip
   hipError_t e = hipSuccess;
   const SeqArgs& f = a.f;
   // 128 query rows a workgroup where that makes two for each compute unit, else 64 (32 utterances of up to 400 rows, 4 heads, f32: both kernels
-  // 156 / 128 us with 128 / 64; 4 sequences of up to 2048, 32 heads of 128, bf16: 281 / 295)
+  // 135 / 113 us with 128 / 64; 4 sequences of up to 2048, 32 heads of 128, bf16: 256 / 269)
   const long long wgs = ((long long)f.rows_q / 128 + (f.batch < f.rows_q ? f.batch : f.rows_q)) * f.heads;
   if (f.rows_q > 0) e = wgs >= 2LL * cus ? grad_q<T, DP, 4, 1>(a, s) : grad_q<T, DP, 2, 2>(a, s);
   if (e != hipSuccess || f.rows_k == 0) return e;
-  // Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 208 -> 174 us
-  // for dK and dV), two of them and twice the workgroups a unit where they pass few (the f32 case 78 -> 65); rows of 512 bytes leave room for two
+  // Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 256 / 294 us
+  // with four / two), two of them and twice the workgroups a unit where they pass few (the f32 case 124 / 113); rows of 512 bytes leave room for two
   const long long turns = (long long)f.rows_q / f.batch * (f.heads / f.kv_heads) / 32;
   if (sizeof(T) * DP <= 256 && turns >= 32) return grad_kv<T, DP, 2, (sizeof(T) * DP > 256 ? 2 : 4)>(a, s);
   return grad_kv<T, DP, 2, 2>(a, s);

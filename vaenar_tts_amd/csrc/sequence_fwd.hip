@@ -4,11 +4,18 @@
 //   S' = K Q'   (keys along the product's rows, the 32 query rows of a tile along its columns: a lane owns ONE query row, its maximum and
 //               sum are register arithmetic plus one exchange with the lane 32 away)
 //   P  = exp2(c S - c m), c = scale log2 e; m is a running bound of the row: it moves only when a tile exceeds it by more than 8 / c, so that
-//        the accumulators are rarely rescaled.  P is rounded to the operands' type (relative 2^-9 / 2^-12, nothing in 32 bits) for the second
-//        product; the row sums take the unrounded values, in 32 bits
+//        the accumulators are rarely rescaled.  P is rounded to the operands' type (by at most 2^-8 / 2^-11 of its value, nothing in 32 bits)
+//        for the second product, as the values of V are; where memory or latency bounds the launch (over a cache with up to 64 rows, packed with
+//        32) what that rounding left goes through a second product.  The row sums take the unrounded values, in 32 bits
 //   O' += V' P'  with P' straight out of the first product's registers (sequence.h: seq_col's key order)
 //
 // K and V tiles come straight from memory to LDS (16 bytes a lane, no registers), the next tile while this one is multiplied.
+//
+// What bounds it: long prompts the matrix pipe and the exponentials between its products (4 prompts of up to 4096 rows, 32 heads of 128, bf16, causal:
+// 417 us = 0.94 PFLOP/s of the products that are not masked; the pipe is busy 41 % of the time, its waves wait 43 %: for the barrier of a tile and
+// for each other's turns on the vector units); a decoding step memory (64 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16: 118 us =
+// 4.7 TB/s, 2 of 100000 keys 139 us = 5.6; a large copy reaches 5.0); few short sequences the way through one workgroup (4 utterances of up to
+// 101 rows: 9.6 us; the append of 8 rows, three loads that wait for each other and one store, takes 4.4).
 #include "sequence.h"
 
 namespace vnr {
@@ -432,9 +439,9 @@ template <typename T> hipError_t fwd(const SeqArgs& a, const SeqPlan& p, hipStre
 
 // Rows a workgroup.  Packed: 128 (every key tile is read once for them) where that makes two workgroups for each compute unit; else 64, else 32
 // with all four waves along the keys: a launch of few workgroups lasts as long as one of them (4 utterances of up to 101 rows, 4 heads, f32:
-// 15.2 / 11.0 / 9.2 us with 128 / 64 / 32 rows; 16 of up to 800, f16: 21.4 / 20.3 / 24.8; 4 prompts of up to 4096, 32 heads of 128, bf16:
-// 424 / 561 / 1052).  Over a cache: 64 rows where no sequence has more (group x new rows), else 128 (one row for each of 64 sequences:
-// 118.9 / 121.6 us with 64 / 128; chunks of up to 512: 229 / 187), and the keys are cut where the tiles alone leave compute units idle: two
+// 15.8 / 11.1 / 9.8 us with 128 / 64 / 32 rows; 16 of up to 800, f16: 20.2 / 18.6 / 26.2; 4 prompts of up to 4096, 32 heads of 128, bf16:
+// 417 / 514 / 1138).  Over a cache: 64 rows where no sequence has more (group x new rows), else 128 (one row for each of 64 sequences:
+// 117.6 / 119.0 us with 64 / 128; chunks of up to 512: 250 / 182), and the keys are cut where the tiles alone leave compute units idle: two
 // workgroups for each of them, no piece shorter than 256 keys (1 row over 100000 keys, 2 sequences: 160 us with one for each, 138 with two).
 SeqPlan seq_plan(const SeqArgs& a, int cus) {
   SeqPlan p;
