@@ -684,3 +684,168 @@ def test_prompt_then_chunks_then_single_rows(eng, kind):
     whole = {n: np.concatenate([np.concatenate(kept[n][b]) for b in range(2)]) for n in kept}
     want = definition(value(whole["q"]), value(whole["k"]), value(whole["v"]), cu, cu, True, D ** -0.5, u)
     close(whole["out"], want["out"], "out", kind)
+
+
+MANY = [
+    # sequences, longest, heads, kv_heads, head_dim, causal: more than one look at the starts; more workgroups than the chip holds, in the order of their lengths
+    (70, 9, 2, 1, 64, True),
+    (150, 40, 1, 1, 64, False),
+    (64, 150, 16, 4, 64, True),
+    (21, 200, 16, 2, 128, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("case", MANY, ids=[str(i) for i in range(len(MANY))])
+def test_many_sequences(eng, case, kind):
+    n, longest, H, G, D, causal = case
+    u = KINDS[kind][1]
+    r = np.random.default_rng(n)
+    lens = r.integers(0, longest + 1, n)
+    lens[n // 3] = 0
+    cu = starts(lens, 1)
+    rows = cu[-1] + 1
+    q, k, v, do = (normal(r, kind, rows, h, D) for h in (H, G, G, H))
+    want = definition(value(q), value(k), value(v), cu, cu, causal, D ** -0.5, u, dout=value(do))
+    d, c = [eng.to_device(x) for x in (q, k, v, do)], eng.to_device(cu)
+    zeros = lambda x: eng.to_device(np.zeros(x.shape, x.dtype))
+    out, lse, grads = zeros(q), eng.to_device(np.zeros((H, rows), np.float32)), [zeros(q), zeros(k), zeros(v)]
+    sequence.packed_attention(eng, *d[:3], c, causal=causal, out=out, lse=lse)
+    sequence.packed_attention_grad(eng, d[3], *d[:3], out, lse, c, causal=causal, dq=grads[0], dk=grads[1], dv=grads[2])
+    for name, a in (("out", out), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
+        got = a.numpy()
+        close(got, want[name], name, kind)
+        assert (got[0] == 0).all() and (got[-1] == 0).all()
+    if not causal:
+        return
+    # the same as one chunk of every sequence over a cache
+    P = 16
+    table, pages = layout(r, lens, P)
+    cache = sequence.PagedCache.empty(eng, pages, G, P, D, KINDS[kind][0])
+    ctx, t = eng.to_device(np.zeros(n, np.int32)), eng.to_device(table)
+    cache.append(d[1], d[2], c, ctx, t)
+    chunk = zeros(q)
+    cache.attend(d[0], c, ctx, t, max_new=int(lens.max()), max_context=int(lens.max()), out=chunk)
+    close(chunk.numpy(), want["out"], "chunk", kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ld", [1 << 23, 1 << 25])              # rows by a lane's 32-bit offset, and by whole addresses
+def test_rows_far_apart(eng, ld):
+    """Offsets that pass 32 bits in bytes and in elements: 300 / 75 rows of 16 / 64 MB."""
+    H, G, D = 4, 2, 64
+    lens = [37, 3, 35] if ld > 1 << 24 else [220, 41, 39]
+    cu = starts(lens)
+    n = cu[-1]
+    r = np.random.default_rng(ld)
+    x, do = normal(r, "f16", n, (H + 2 * G) * D), normal(r, "f16", n, H, D)
+    far = eng.empty((n, ld), np.float16)
+    for i in range(n):
+        far.view(i * ld, x[i].shape).copy_from(x[i])
+    cut = lambda o, h: value(x[:, o:o + h * D]).reshape(n, h, D)
+    want = definition(cut(0, H), cut(H * D, G), cut((H + G) * D, G), cu, cu, True, D ** -0.5, KINDS["f16"][1], dout=value(do))
+    a = [far.view(0, (n, H, D)), far.view(H * D, (n, G, D)), far.view((H + G) * D, (n, G, D))]
+    c, strides = eng.to_device(cu), dict(ldq=ld, ldk=ld, ldv=ld)
+    out, lse = sequence.packed_attention(eng, *a, c, **strides)
+    grads = sequence.packed_attention_grad(eng, eng.to_device(do), *a, out, lse, c, **strides)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+        close(got.numpy(), want[name], name, "f16")
+
+
+@pytest.mark.gpu
+def test_pages_far_apart(eng):
+    """A pool of more than 2^31 elements: its last pages hold the sequences."""
+    G, H, P, D, pages = 2, 4, 64, 128, 140000
+    lens = [150, 1, 64]
+    r = np.random.default_rng(3)
+    table, used = layout(r, lens, P, spare=0)
+    table[table >= 0] += pages - used
+    cu = starts(lens)
+    n = cu[-1]
+    q, k, v = (normal(r, "bf16", n, h, D) for h in (H, G, G))
+    want = definition(value(q), value(k), value(v), cu, cu, True, D ** -0.5, KINDS["bf16"][1])
+    cache = sequence.PagedCache(eng, eng.empty((pages, G, P, D), np.uint16), eng.empty((pages, G, P, D), np.uint16))
+    c, ctx, t = eng.to_device(cu), eng.to_device(np.zeros(3, np.int32)), eng.to_device(table)
+    cache.append(eng.to_device(k), eng.to_device(v), c, ctx, t)
+    out = cache.attend(eng.to_device(q), c, ctx, t, max_new=150, max_context=150)
+    close(out.numpy(), want["out"], "out", "bf16")
+    last = eng.to_device(np.int32([0, 1, 2, 3]))                 # a single row of every sequence
+    ql = q[cu[1:] - 1]
+    one = cache.attend(eng.to_device(ql), last, eng.to_device(np.int32(lens) - 1), t, max_new=1, max_context=150)
+    close(one.numpy(), (want["out"][0][cu[1:] - 1], want["out"][1][cu[1:] - 1]), "single rows", "bf16")
+
+
+@pytest.mark.gpu
+def test_two_engines_in_turn(eng):
+    """Calls of two handles on their own streams, in flight at once: neither's workspace is the other's."""
+    other = _lib.Engine(tiny_hps(), 0)
+    try:
+        results = []
+        for turn in range(2):
+            held = []
+            for e, seed in ((eng, 1), (other, 2)):
+                r = np.random.default_rng(seed)
+                cu = starts([300, 20, 133])
+                x = [e.to_device(normal(r, "bf16", cu[-1], h, 64)) for h in (8, 2, 2, 8)]
+                kp, vp = (e.to_device(normal(r, "bf16", 40, 2, 64, 64)) for _ in range(2))
+                held.append((e, x, e.to_device(cu), sequence.PagedCache(e, kp, vp), e.to_device(starts([1, 1])), e.to_device(np.int32([1100, 900])),
+                             e.to_device(np.arange(40, dtype=np.int32).reshape(2, 20)), e.to_device(normal(r, "bf16", 2, 8, 64))))
+            got = [[], []]
+            for _ in range(3):
+                for i, (e, (q, k, v, do), c, cache, one, ctx, table, row) in enumerate(held if turn else held[::-1]):
+                    out, lse = sequence.packed_attention(e, q, k, v, c)
+                    got[i if turn else 1 - i] = [cache.attend(row, one, ctx, table, 1, 1200), *sequence.packed_attention_grad(e, do, q, k, v, out, lse, c)]
+            results.append([[a.numpy() for a in g] for g in got])
+        for a, b in zip(*results):
+            assert all((x == y).all() for x, y in zip(a, b))
+        assert (results[0][0][1] != results[0][1][1]).any()
+    finally:
+        other.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_batches_without_keys_or_without_rows(eng, kind):
+    H, G, D = 4, 2, 64
+    r = np.random.default_rng(12)
+    x, y = normal(r, kind, 5, H, D), normal(r, kind, 7, G, D)
+    fill = lambda *s: eng.to_device(store(np.full(s, 7, np.float32), kind))
+    none, five, seven = (eng.to_device(np.int32(c)) for c in ([0, 0, 0], [0, 2, 5], [0, 0, 7]))
+    nothing = lambda h: eng.empty((0, h, D), x.dtype)
+    q, out, lse, dq = eng.to_device(x), fill(5, H, D), eng.to_device(np.full((H, 5), 7, np.float32)), fill(5, H, D)
+    sequence.packed_attention(eng, q, nothing(G), nothing(G), five, none, True, None, out, lse)
+    assert (out.numpy() == 0).all() and (lse.numpy() == -np.inf).all()
+    sequence.packed_attention_grad(eng, q, q, nothing(G), nothing(G), out, lse, five, none, dq=dq, dk=nothing(G), dv=nothing(G))
+    assert (dq.numpy() == 0).all()
+    k, dk, dv, empty = eng.to_device(y), fill(7, G, D), fill(7, G, D), eng.empty((H, 0))
+    sequence.packed_attention(eng, nothing(H), k, k, none, seven, False, None, nothing(H), empty)
+    sequence.packed_attention_grad(eng, nothing(H), nothing(H), k, k, nothing(H), empty, none, seven, False, dq=nothing(H), dk=dk, dv=dv)
+    assert (dk.numpy() == 0).all() and (dv.numpy() == 0).all()
+    cache = sequence.PagedCache(eng, fill(3, G, 16, D), fill(3, G, 16, D))
+    ctx, table = eng.to_device(np.int32([3, 4])), eng.to_device(np.int32([[0], [1]]))
+    cache.append(nothing(G), nothing(G), none, ctx, table)
+    assert cache.attend(nothing(H), none, ctx, table, 1, 16).numpy().shape == (0, H, D)
+    assert (value(cache.k.numpy()) == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 70])
+def test_positions_behind_the_bound_are_not_seen(eng, new):
+    """max_context below a sequence's length: every row sees the positions in front of the bound; a context that is no length counts as the bound."""
+    H, G, D, P, bound = 4, 2, 64, 16, 600
+    r = np.random.default_rng(new)
+    total = [900, bound + 40]
+    table, pages = layout(r, total, P)
+    kc, vc = normal(r, "f16", pages, G, P, D), normal(r, "f16", pages, G, P, D)
+    ctx = [total[0] - new, total[1] - new]
+    held = lambda c: np.concatenate([c[table[b, :-(-bound // P)]].transpose(0, 2, 1, 3).reshape(-1, G, D)[:bound] for b in range(2)])
+    cu = starts([new, new])
+    q = normal(r, "f16", cu[-1], H, D)
+    want = definition(value(q), value(held(kc)), value(held(vc)), cu, starts([bound, bound]), True, D ** -0.5, KINDS["f16"][1], first=ctx)
+    cache = sequence.PagedCache(eng, eng.to_device(kc), eng.to_device(vc))
+    for contexts in (ctx, [2 ** 31 - 1, ctx[1]]):
+        if contexts is not ctx:
+            want = definition(value(q), value(held(kc)), value(held(vc)), cu, starts([bound, bound]), True, D ** -0.5, KINDS["f16"][1], first=[bound, ctx[1]])
+        out = cache.attend(eng.to_device(q), eng.to_device(cu), eng.to_device(np.int32(contexts)), eng.to_device(table), new, bound)
+        close(out.numpy(), want["out"], "out", "f16")

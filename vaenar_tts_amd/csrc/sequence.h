@@ -293,7 +293,7 @@ __device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total
     int n = e - s;
     int t = (int)(((long long)n * mult + rows - 1) / rows);
     if (gridDim.x > 512 && batch > 1 && batch <= 64) {       // ranks, then everything to the lane of its rank
-      const int key = b < batch ? n + (two ? 0 : x0) : -1;
+      const int key = b < batch ? n + (two ? 0 : x0 < 1 << 30 ? x0 : 1 << 30) : -1;
       int rank = 0;
       for (int j = 0; j < batch; ++j) { const int k = __builtin_amdgcn_readlane(key, j); rank += (k > key || (k == key && j < lane)) ? 1 : 0; }
       rank = b < batch ? rank : lane;

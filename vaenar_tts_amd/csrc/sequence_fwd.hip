@@ -14,7 +14,7 @@
 // What bounds it: long prompts the matrix pipe and the exponentials between its products (4 prompts of up to 4096 rows, 32 heads of 128, bf16, causal:
 // 417 us = 0.94 PFLOP/s of the products that are not masked; the pipe is busy 41 % of the time, its waves wait 43 %: for the barrier of a tile and
 // for each other's turns on the vector units); a decoding step memory (64 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16: 118 us =
-// 4.7 TB/s, 2 of 100000 keys 139 us = 5.6; a large copy reaches 5.0); few short sequences the way through one workgroup (4 utterances of up to
+// 4.7 TB/s, 2 of 100000 keys 140 us = 5.5; a large copy reaches 5.0); few short sequences the way through one workgroup (4 utterances of up to
 // 101 rows: 9.6 us; the append of 8 rows, three loads that wait for each other and one store, takes 4.4).
 #include "sequence.h"
 
