@@ -849,3 +849,61 @@ def test_positions_behind_the_bound_are_not_seen(eng, new):
             want = definition(value(q), value(held(kc)), value(held(vc)), cu, starts([bound, bound]), True, D ** -0.5, KINDS["f16"][1], first=[bound, ctx[1]])
         out = cache.attend(eng.to_device(q), eng.to_device(cu), eng.to_device(np.int32(contexts)), eng.to_device(table), new, bound)
         close(out.numpy(), want["out"], "out", "f16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("power", [-14, 12])
+@pytest.mark.parametrize("large", ["k", "q"])
+def test_gradients_follow_a_power_of_two_on_dout(eng, large, power, dim, kind):
+    """The gradient is linear in dout, and a power of two on dout is one on every product and sum of it: where a result is an ordinary number of
+    the type both times it is the same but for one step, however small (long rows, dout of 1e-4) or large (beyond float16's 65504) dS is on
+    the way.  Large keys and small queries keep dQ inside the type's range, the other way round dK.  Tolerance: half a step for the rounding of either
+    result, and for the sums in 32 bits behind each the definition's bound with u = 0 (the matrix instructions round products of subnormal float16
+    operands, dout of 1e-4, otherwise than the same products a power of two higher)."""
+    r = np.random.default_rng(dim + power)
+    cu = starts([700, 65, 3, 2000])
+    n, H, G = cu[-1], 4, 2
+    up = 2.0 ** (8 if power < 0 else -8)
+    fq, fk = (1 / up, up) if large == "k" else (up, 1 / up)
+    q, k = (store(value(normal(r, kind, n, h, dim)) * f, kind) for h, f in ((H, fq), (G, fk)))
+    v = store(value(normal(r, kind, n, G, dim)) * 8, kind)
+    dout = value(store(np.round(r.standard_normal((n, H, dim)).clip(-3.9, 3.9) * 512) / 512, kind))      # exact at both sizes
+    d, c = [eng.to_device(x) for x in (q, k, v)], eng.to_device(cu)
+    out, lse = sequence.packed_attention(eng, *d, c)
+    got = []
+    for f in (1.0, 2.0 ** power):
+        do = store(dout * f, kind)
+        assert (value(do) == dout * f).all()
+        got.append([value(x.numpy()) for x in sequence.packed_attention_grad(eng, eng.to_device(do), *d, out, lse, c)])
+    least, most = {"f16": (2.0 ** -14, 65504.0)}.get(kind, (2.0 ** -120, 2.0 ** 120))
+    sums = None
+    for name, one, two in zip(("dq", "dk", "dv"), *got):
+        want = one * 2.0 ** power
+        size = np.abs(want)
+        assert np.isfinite(one).all() and np.isfinite(two[size < 0.99 * most]).all(), name
+        both = (np.abs(one) > least) & (size > least) & (size < 0.99 * most)      # (at the least ordinary number a rounding may come from the finer steps below)
+        if (two[both] != want[both]).any():
+            sums = sums or definition(value(q), value(k), value(v), cu, cu, True, np.float64(np.float32(dim ** -0.5)), 0.0, dout=dout)
+            tol = 2 * KINDS[kind][1] * size + 2 * sums[name][1] * 2.0 ** power
+            assert (np.abs(two - want)[both] <= tol[both]).all(), name
+        if name == {"k": "dq", "q": "dk"}[large]:
+            assert both.mean() > 0.8                              # (the case is about these)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_gradients_whose_differences_pass_the_range_of_float16(eng, dim):
+    """P (dP - delta) beyond 65504 where dQ, dK and dV are ordinary float16 numbers."""
+    r = np.random.default_rng(dim)
+    cu = starts([300, 40])
+    n, H, G = cu[-1], 4, 2
+    u = KINDS["f16"][1]
+    q, k, v, do = (store(r.standard_normal((n, h, dim)) * f, "f16") for h, f in ((H, 1), (G, 1), (G, 8), (H, 1500)))
+    want = definition(value(q), value(k), value(v), cu, cu, True, np.float64(np.float32(dim ** -0.5)), u, dout=value(do))
+    assert max(np.abs(want[x][0]).max() for x in ("dq", "dk", "dv")) < 65000
+    d, c = [eng.to_device(x) for x in (q, k, v)], eng.to_device(cu)
+    out, lse = sequence.packed_attention(eng, *d, c)
+    for name, got in zip(("dq", "dk", "dv"), sequence.packed_attention_grad(eng, eng.to_device(do), *d, out, lse, c)):
+        close(got.numpy(), want[name], name, "f16")

@@ -6,6 +6,8 @@
 // P is rounded once to the operands' type for dV (as dout is); what that rounding leaves of dS goes through a second product in 16-bit types --
 // the differences dP - delta cancel, and a rounding of what is left shows in dQ and dK (with it they are within 1.1 of the error of a plain
 // form in 32 bits whose results are rounded once, dV within 1.4).  Every sum is held in 32 bits.
+// float16 holds 2^-24 .. 65504, dS anything (dout of 1e-4 over 2000 keys is below, dout of 1500 above): it is multiplied by a power of two
+// that fits the largest of its row (dQ) or key (dK) so far, a running bound as the forward's of the logits, and the sums are divided by it at the end.
 //
 // What bounds it: 4 sequences of up to 2048 rows, 32 heads over 8 of 128, bf16, causal: 256 us, 106 for dQ and 171 for dK and dV -- nine products
 // where the formulas have five, 0.79 PFLOP/s of them; a workgroup of dK and dV lasts as long as the rows that see its keys.  32 utterances of
@@ -45,6 +47,28 @@ template <typename T, int DP> struct Rows {                    // (`first` is th
     }
   }
 };
+
+// The columns of dS as float16 operands: x holds 2^lift of them, and where that passes 2^15 the column's lift comes down to where its largest is
+// 2^10 .. 2^11 -- `acc`, what went through the second product before, with it.  (What the second half's smallest step, 2^-25, leaves out is 2^-35 of a
+// column's largest.  Both lanes of a column, 32 apart, take the same turn; a value that is not finite moves nothing.  In float16 the bf16 case above
+// takes 275 us with it, 261 without, the f32 one 41 and 38.)
+constexpr int kLift = 60;                                    // at first: 2^60 times what float16 operands make of dP stays a 32-bit number
+template <int N> __device__ __forceinline__ void fit(f32x16& x, int& lift, f32x16 (&acc)[N]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, __builtin_fabsf(x[i]));
+  top = seq_pair_max(top);
+  if (__builtin_amdgcn_ballot_w64(top > 32768.f)) {
+    const int e = 11 - __builtin_amdgcn_frexp_expf(top), down = top > 32768.f && e < 0 ? e : 0;
+    lift += down;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], down);
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], down);
+  }
+}
 
 // 32 RG query rows of one head; KS key groups of waves, as in the forward kernel.  Leaves delta and lse log2 e of its rows for the other
 // kernel: delta [2][heads][rows_q].
@@ -144,6 +168,8 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
     delta = seq_pair_sum(sum);
   }
   if (live && g == 0 && kg == 0) { ga.delta[place] = delta; ga.delta[(long long)a.heads * a.rows_q + place] = lse2; }
+  constexpr bool kFit = __is_same(T, _Float16);
+  int lift = kFit ? kLift : 0;
   int k0 = (kg - KS) * BN, stage = 0;                        // (the first turn only fetches)
   for (int kt = -step; kt < some; kt += step, k0 += step, stage ^= kStage) {
     seq_dma_wait();
@@ -161,11 +187,15 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
       f32x16 s, p;
       products(tk, j, s, p);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2)) * (p[i] - delta);
+      for (int i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
+        s[i] = x * (kFit ? __builtin_amdgcn_ldexpf(p[i] - delta, lift) : p[i] - delta);
+      }
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = k0 + 32 * j + 8 * (i >> 2) + 4 * g + (i & 3) < limit ? s[i] : 0.f;
       }
+      if constexpr (kFit) fit(s, lift, acc);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if constexpr (sizeof(T) == 2) {
@@ -184,6 +214,12 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
         }
       }
     }
+  }
+  if constexpr (kFit) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], -lift);
   }
   if (KS > 1) {                                              // the key groups' parts of the same rows, summed in the groups' order
     __syncthreads();
@@ -270,6 +306,8 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
   seq_settle(kf); seq_settle(vf);
   // ---- one tile of rows: the two products, the weights and their gradients, what they add to dV and dK ----------------------------------------
   f32x16 s, p;
+  constexpr bool kFit = __is_same(T, _Float16);
+  int lift = kFit ? kLift : 0;
   SeqReads<T, DP> reads;
   reads.set(lane);
   auto products = [&](unsigned tile) {
@@ -291,7 +329,7 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * q + e;
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[e]));
-        p[i] = x * (p[i] - de[e]);
+        p[i] = x * (kFit ? __builtin_amdgcn_ldexpf(p[i] - de[e], lift) : p[i] - de[e]);
         s[i] = x;
       }
     }
@@ -349,7 +387,14 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
     products(lds + stage);
     weights(lds + stage);
     if (a.causal && row + ahead < kw + 31) masks(row);
+    if constexpr (kFit) fit(p, lift, dk);
     sums(lds + stage);
+  }
+  if constexpr (kFit) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[d][i] = __builtin_amdgcn_ldexpf(dk[d][i], -lift);
   }
   if (HG > 1) {                                              // the row groups' sums, in their order: dK, then dV through the same buffer
     constexpr int N = (DP / 32) * 16;
