@@ -907,3 +907,60 @@ def test_gradients_whose_differences_pass_the_range_of_float16(eng, dim):
     out, lse = sequence.packed_attention(eng, *d, c)
     for name, got in zip(("dq", "dk", "dv"), sequence.packed_attention_grad(eng, eng.to_device(do), *d, out, lse, c)):
         close(got.numpy(), want[name], name, "f16")
+
+
+FEW = [
+    # lens of queries, of keys (None: the same), heads, kv_heads, head_dim
+    ([64], None, 8, 2, 128),
+    ([65], None, 8, 2, 128),
+    ([300, 1, 129, 66], None, 8, 2, 64),
+    ([90, 400], [5, 333], 4, 1, 80),                              # rows that see nothing in front of the first ones that see something
+    ([700, 650, 700, 700], None, 80, 8, 128),                     # the launch of many rows
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("case", FEW, ids=[str(i) for i in range(len(FEW))])
+def test_dq_of_rows_that_see_few_keys(eng, case, kind):
+    """delta = sum_d dO out with the rounded `out` reaches every dS of its row, and where few keys share the weight nothing averages it away: rows
+    that see up to 64 keys take sum_j P dP, however long their sequence is.  Tolerance: no step of the type but the result's own,
+      dS   (u^2 + 2 e_s + 32 h) |dS| + 2^-32 max|dS| + P (e_dP + e_delta),   e_delta = (2 e_s + (n + 48) h) sum P |dP| + sum P e_dP
+    (dS goes in two halves: u^2; float16's smallest step against the row's largest; delta is a sum in 32 bits)."""
+    lq, lk, H, G, D = case
+    u = KINDS[kind][1]
+    r = np.random.default_rng(sum(lq))
+    cu_q = starts(lq)
+    cu_k = cu_q if lk is None else starts(lk)
+    q, k, v, do = (normal(r, kind, n, h, D) for n, h in ((cu_q[-1], H), (cu_k[-1], G), (cu_k[-1], G), (cu_q[-1], H)))
+    d = [eng.to_device(x) for x in (q, k, v, do)]
+    cq, ck = eng.to_device(cu_q), eng.to_device(cu_k)
+    out, lse = sequence.packed_attention(eng, *d[:3], cq, ck)
+    got = value(sequence.packed_attention_grad(eng, d[3], *d[:3], out, lse, cq, ck)[0].numpy())
+    q, k, v, do = (value(x) for x in (q, k, v, do))
+    scale, checked = np.float64(np.float32(D ** -0.5)), 0
+    for b in range(len(lq)):
+        ahead = (cu_k[b + 1] - cu_k[b]) - (cu_q[b + 1] - cu_q[b])
+        first = max(0, -ahead)                                    # the first row that sees a key
+        rows = cu_q[b] + np.arange(first, min(cu_q[b + 1] - cu_q[b], 64 - ahead))
+        nk = min(64, cu_k[b + 1] - cu_k[b])
+        if len(rows) == 0:
+            continue
+        see = np.arange(nk) <= (rows - cu_q[b] + ahead)[:, None]
+        for h in range(H):
+            K, V = (x[cu_k[b]:cu_k[b] + nk, h // (H // G)] for x in (k, v))
+            Q, dO = q[rows, h], do[rows, h]
+            x = np.where(see, Q @ K.T * scale, -np.inf)
+            e_s = (D + 4) * H24 * scale * np.where(see, np.abs(Q) @ np.abs(K).T, 0).max()
+            p = np.exp(x - x.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            dP, e_dP = dO @ V.T, (D + 4) * H24 * (np.abs(dO) @ np.abs(V).T)
+            dS = p * (dP - (p * dP).sum(1, keepdims=True))
+            e_delta = (2 * e_s + (nk + 48) * H24) * (p * np.abs(dP)).sum(1, keepdims=True) + (p * e_dP).sum(1, keepdims=True)
+            e_dS = (u * u + 2 * e_s + 32 * H24) * np.abs(dS) + 2.0 ** -32 * np.abs(dS).max(1, keepdims=True) + p * (e_dP + e_delta)
+            want = scale * dS @ K
+            tol = u * np.abs(want) + scale * ((e_dS + (nk + 16) * H24 * np.abs(dS)) @ np.abs(K)) + TINY
+            off = np.abs(got[rows, h] - want) - tol
+            assert off.max() <= 0, (b, h, rows[off.max(1) > 0] - cu_q[b], off.max())
+            checked += len(rows)
+    assert checked

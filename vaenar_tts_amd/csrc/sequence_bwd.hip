@@ -140,14 +140,17 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
       p = seq_mma(seq_row<T, DP>(tk, BN + 32 * j, t), df[t], p);           // (V lies behind K)
     }
   };
-  // The rounding of `out` reaches dS through delta, and where few keys share a row's weight nothing averages it away (rows of up to 8 keys: dQ 1.7
-  // times as far from 64 bits as a plain form's).  Up to 64 keys: delta = sum_j P dP instead, in a turn of its own.
-  if (sizeof(T) == 2 && nk <= 64) {
+  // The rounding of `out` reaches dS through delta, and where few keys share a row's weight nothing averages it away (rows of two keys: dQ twice as
+  // far from 64 bits as a plain form's, of eight 1.2 times).  Rows that see up to 64 keys take delta = sum_j P dP instead, in turns of their own
+  // over these keys: whole short sequences, of a causal one the workgroup that holds its first rows.
+  constexpr int kFew = 64;
+  if (sizeof(T) == 2 && seen(r0) <= kFew) {
     float sum = 0.f;
-    for (int kt = -BN, stage = 0; kt < some; kt += BN, stage ^= kStage) {
+    const int end = some < kFew ? some : kFew;
+    for (int kt = -BN, stage = 0; kt < end; kt += BN, stage ^= kStage) {
       seq_dma_wait();
       __syncthreads();
-      if (kt + BN < some) {
+      if (kt + BN < end) {
         const unsigned t = lds + (stage ^ kStage);
         rk.template fetch<kIssue>(kb, kt + BN, BN, rg * kIssue, t, lane);
         rv.template fetch<kIssue>(vb, kt + BN, BN, rg * kIssue, t + kTile, lane);
@@ -165,7 +168,8 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
         }
       }
     }
-    delta = seq_pair_sum(sum);
+    sum = seq_pair_sum(sum);
+    delta = limit <= kFew ? sum : delta;
   }
   if (live && g == 0 && kg == 0) { ga.delta[place] = delta; ga.delta[(long long)a.heads * a.rows_q + place] = lse2; }
   constexpr bool kFit = __is_same(T, _Float16);
