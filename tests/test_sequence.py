@@ -964,3 +964,41 @@ def test_dq_of_rows_that_see_few_keys(eng, case, kind):
             assert off.max() <= 0, (b, h, rows[off.max(1) > 0] - cu_q[b], off.max())
             checked += len(rows)
     assert checked
+
+
+def tail(n, D, r):
+    """One key whose weight is 2^25.5 times that of each of n - 1 others, and a value of zero: the result is made of the others alone."""
+    q = np.zeros((1, D))
+    q[0, 0] = 1
+    k, v = np.zeros((n, D)), 1 + 0.25 * r.standard_normal((n, D))
+    k[0, 0], v[0] = np.float16(25.5 * np.log(2)), 0
+    return q, k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [1, 160])
+def test_small_weights_of_float16_reach_the_result(eng, heads, dim):
+    """Weights far below the row's largest are what the row sum counts, so the result has to count them too: in float16 each is rounded by half a step
+    of its own, or by 2^-36 of the row's largest."""
+    r = np.random.default_rng(dim)
+    n, new, u, P = 4096, 130, KINDS["f16"][1], 64
+    q1, k1, v1 = tail(n, dim, r)
+    q, k, v = store(np.broadcast_to(q1, (n, heads, dim)), "f16"), store(k1[:, None], "f16"), store(v1[:, None], "f16")
+    c, ident = eng.to_device(starts([n])), eng.to_device(np.arange(n // P, dtype=np.int32)[None])
+    one = definition(value(q)[:1, :1], value(k), value(v), starts([1]), starts([n]), False, 1.0, u)
+    w, tol = (x[0, 0] for x in one["out"])
+    tol = tol + n * 2.0 ** -36 * np.abs(value(v)).max()
+    assert (np.abs(w) > 100 * tol).all() and (np.abs(w) > 2.0 ** -14).all()
+    got = {}
+    for rows in (1, 40, n) if heads == 1 else (n,):
+        cq = eng.to_device(starts([rows]))
+        o, _ = sequence.packed_attention(eng, eng.to_device(q[:rows]), eng.to_device(k), eng.to_device(v), cq, c, causal=False, scale=1.0)
+        got["packed", rows] = value(o.numpy())
+    paged = lambda x: eng.to_device(np.ascontiguousarray(x.reshape(n // P, P, 1, dim).transpose(0, 2, 1, 3)))
+    cache = sequence.PagedCache(eng, paged(k), paged(v))
+    for rows in (1, new):
+        o = cache.attend(eng.to_device(q[:rows]), eng.to_device(starts([rows])), eng.to_device(np.int32([n - 1])), ident, rows, n, scale=1.0)
+        got["cache", rows] = value(o.numpy())
+    for name, x in got.items():
+        assert (np.abs(x - w) <= tol + TINY).all(), (name, x[0, 0, :4], w[:4])

@@ -4,9 +4,10 @@
 //   S' = K Q'   (keys along the product's rows, the 32 query rows of a tile along its columns: a lane owns ONE query row, its maximum and
 //               sum are register arithmetic plus one exchange with the lane 32 away)
 //   P  = exp2(c S - c m), c = scale log2 e; m is a running bound of the row: it moves only when a tile exceeds it by more than 8 / c, so that
-//        the accumulators are rarely rescaled.  P is rounded to the operands' type (by at most 2^-8 / 2^-11 of its value, nothing in 32 bits)
-//        for the second product, as the values of V are; where memory or latency bounds the launch (over a cache with up to 64 rows, packed with
-//        32) what that rounding left goes through a second product.  The row sums take the unrounded values, in 32 bits
+//        the accumulators are rarely rescaled (in float16 by more than 4 / c, see Weight).  P is rounded to the operands' type (by at most 2^-8 of its
+//        value, in float16 2^-11 of it or 2^-36 of the row's largest; nothing in 32 bits) for the second product, as the values of V are; where memory
+//        or latency bounds the launch (over a cache with up to 64 rows, packed with 32) what that rounding left goes through a second product.  The
+//        row sums take the unrounded values, in 32 bits
 //   O' += V' P'  with P' straight out of the first product's registers (sequence.h: seq_col's key order)
 //
 // K and V tiles come straight from memory to LDS (16 bytes a lane, no registers), the next tile while this one is multiplied.
@@ -22,7 +23,10 @@ namespace vnr {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kBound = 8.f;                                // how far (log2) a row may exceed its running bound before it is moved
+// How far (log2) a row may exceed its running bound before it is moved, and the power of two that its weights carry.  float16 has no weights of its own
+// precision below 2^-14 and none below 2^-25: there they are 2^11 times what they are elsewhere (at most 2^15 with the slack of the bound), so that those
+// down to 2^-25 of the largest are rounded like any other and what is lost of the rest is 2^-36 of it.
+template <typename T> struct Weight { static constexpr float kSlack = __is_same(T, _Float16) ? 4.f : 8.f, kLift = __is_same(T, _Float16) ? 11.f : 0.f, kTimes = __is_same(T, _Float16) ? 2048.f : 1.f; };
 constexpr int kMaxSplits = 64;
 
 // Where the rows of a task's keys and values are.  `n`: keys of the sequence; rows from n on read as zeros.  A whole tile goes by scalar
@@ -105,11 +109,13 @@ struct Fwd {
   static_assert(kJoin <= 2 * KS * kStage, "the join lies where the tiles were");
 };
 
-// A row's bound in units of log2, rounded once and the same wherever it is used: weights of different tiles stay in proportion
-__device__ __forceinline__ float bound(float m, float c) {
+// What is taken off a row's logits in units of log2, rounded once and the same wherever it is used: weights of different tiles stay in proportion
+template <typename T> __device__ __forceinline__ float bound(float m, float c) {
 #pragma clang fp contract(off)
-  return m * c;
+  return m * c - Weight<T>::kLift;
 }
+// the same without the weights' power of two (an exact sum: the bound lies on its own, coarser grid or is the exact difference)
+template <typename T> __device__ __forceinline__ float bare(float bound) { return bound + Weight<T>::kLift; }
 
 // The pieces of a row's keys joined by one wave, lanes along the channels
 template <typename T>
@@ -144,7 +150,7 @@ __device__ __forceinline__ void join_row(const SeqArgs& a, long long pr, long lo
       if (s < a.splits && fs != 0.f) { x[0] += fs * p[i][0]; x[1] += fs * p[i][1]; }      // (an empty piece has left nothing)
     }
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / (sum * Weight<T>::kTimes) : 0.f;      // (the pieces' results carry the power of two)
   if (2 * lane < a.dim) {
     T* op = (T*)a.out + token * a.ldo + (long long)head * a.dim + col;
     op[0] = (T)(x[0] * inv); op[1] = (T)(x[1] * inv);
@@ -226,6 +232,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m = -__builtin_inff(), l = 0.f;                      // running bound (of the raw products) and this lane's part of the row sum
   const float c = a.scale * kLog2e;
+  float mc = 0.f;                                            // bound(m, c)
 
   char* base = smem + kg * 2 * F::kStage;
   const unsigned lds = seq_lds(base);
@@ -256,17 +263,17 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
     mx = seq_pair_max(mx);
-    if (__builtin_amdgcn_ballot_w64((mx - m) * c > kBound || (mx > m && m == -__builtin_inff()))) {
+    if (__builtin_amdgcn_ballot_w64((mx - m) * c > Weight<T>::kSlack || (mx > m && m == -__builtin_inff()))) {
       const float m1 = fmaxf(m, mx);
-      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound(m, c) - bound(m1, c));
-      m = m1;
+      const float b1 = m1 == -__builtin_inff() ? 0.f : bound<T>(m1, c);
+      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mc - b1);
+      m = m1; mc = b1;
       l *= f;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= f;
     }
-    const float mc = m == -__builtin_inff() ? 0.f : bound(m, c);
 #pragma unroll
     for (int j = 0; j < F::NJ; ++j)
 #pragma unroll
@@ -341,7 +348,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     for (int k = 0; kg == 0 && k < KS - 1; ++k) {
       const float* y = x + (k * RG + rg) * (N + 2) * 64;
       const float m2 = y[N * 64], l2 = y[(N + 1) * 64], m1 = fmaxf(m, m2);
-      const float mc = bound(m1, c), f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound(m, c) - mc), f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound(m2, c) - mc);
+      const float mc = bound<T>(m1, c), f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound<T>(m, c) - mc), f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound<T>(m2, c) - mc);
       m = m1; l = l * f1 + l2 * f2;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -372,7 +379,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     const long long n = (long long)a.rows_q * a.heads;
     if (live && kg == 0) {
       const long long pr = split * n + (long long)token * a.heads + head;
-      if (g == 0) { const sq_f2 x = {m == -__builtin_inff() ? m : bound(m, c), l}; *reinterpret_cast<sq_f2*>(a.ml + 2 * pr) = x; }
+      if (g == 0) { const sq_f2 x = {m == -__builtin_inff() ? m : bare<T>(bound<T>(m, c)), l * (1.f / Weight<T>::kTimes)}; *reinterpret_cast<sq_f2*>(a.ml + 2 * pr) = x; }
       float* op = a.part + pr * a.dim;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -395,7 +402,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
       if (col < a.dim) seq_store4<T>(op + col, o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv, o[d][i + 3] * inv);
     }
   // the weights are relative to the ROUNDED bound; what its rounding left belongs to the sum
-  if (a.lse && g == 0) a.lse[(long long)head * a.rows_q + token] = l != 0.f ? m * a.scale + (__logf(l) - kLn2 * __builtin_fmaf(m, c, -bound(m, c))) : -__builtin_inff();
+  if (a.lse && g == 0) a.lse[(long long)head * a.rows_q + token] = l != 0.f ? m * a.scale + (__logf(l * (1.f / Weight<T>::kTimes)) - kLn2 * __builtin_fmaf(m, c, -bare<T>(bound<T>(m, c)))) : -__builtin_inff();
 }
 
 template <typename T>
