@@ -1002,3 +1002,21 @@ def test_small_weights_of_float16_reach_the_result(eng, heads, dim):
         got["cache", rows] = value(o.numpy())
     for name, x in got.items():
         assert (np.abs(x - w) <= tol + TINY).all(), (name, x[0, 0, :4], w[:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_weights_of_float16_reach_dv(eng, dim):
+    """512 rows with a weight of 2^-25.5 for each of the later keys: dV of those keys is 2^-25.5 of dout's sum, an ordinary float16 number."""
+    r = np.random.default_rng(dim)
+    n, rows, u = 600, 512, KINDS["f16"][1]
+    q1, k1, v1 = tail(n, dim, r)
+    q, k, v = store(np.broadcast_to(q1, (rows, 1, dim)), "f16"), store(k1[:, None], "f16"), store(v1[:, None], "f16")
+    do = store(1024 * (1 + 0.25 * r.standard_normal((rows, 1, dim))), "f16")
+    cu_q, cu_k = starts([rows]), starts([n])
+    want = definition(value(q), value(k), value(v), cu_q, cu_k, False, 1.0, u, dout=value(do))["dv"]
+    assert (np.abs(want[0][1:]) > 2.0 ** -14).all() and (np.abs(want[0]) < 65504 * 16).all()
+    d, cq, ck = [eng.to_device(x) for x in (q, k, v)], eng.to_device(cu_q), eng.to_device(cu_k)
+    out, lse = sequence.packed_attention(eng, *d, cq, ck, causal=False, scale=1.0)
+    dv = sequence.packed_attention_grad(eng, eng.to_device(do), *d, out, lse, cq, ck, causal=False, scale=1.0)[2]
+    close(dv.numpy()[1:], [x[1:] for x in want], "dv", "f16")

@@ -8,6 +8,7 @@
 // form in 32 bits whose results are rounded once, dV within 1.4).  Every sum is held in 32 bits.
 // float16 holds 2^-24 .. 65504, dS anything (dout of 1e-4 over 2000 keys is below, dout of 1500 above): it is multiplied by a power of two
 // that fits the largest of its row (dQ) or key (dK) so far, a running bound as the forward's of the logits, and the sums are divided by it at the end.
+// P needs no such search, it is at most 1: 2^15 P goes into dV's product (weights below 2^-40 are lost, those from 2^-29 on are rounded like any other).
 //
 // What bounds it: 4 sequences of up to 2048 rows, 32 heads over 8 of 128, bf16, causal: 256 us, 106 for dQ and 171 for dK and dV -- nine products
 // where the formulas have five, 0.79 PFLOP/s of them; a workgroup of dK and dV lasts as long as the rows that see its keys.  32 utterances of
@@ -18,6 +19,7 @@ namespace vnr {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+template <typename T> struct Weight { static constexpr float kLift = __is_same(T, _Float16) ? 15.f : 0.f, kTimes = __is_same(T, _Float16) ? 32768.f : 1.f; };      // of P in dV's product
 
 // Rows of one head in memory, `ld` bytes apart; rows from n on read as zeros.  Whole tiles go by scalar addresses, the last one of a sequence
 // and heads narrower than the tile by an address in every lane (zeros where there is nothing).
@@ -52,7 +54,7 @@ template <typename T, int DP> struct Rows {                    // (`first` is th
 // 2^10 .. 2^11 -- `acc`, what went through the second product before, with it.  (What the second half's smallest step, 2^-25, leaves out is 2^-35 of a
 // column's largest.  Both lanes of a column, 32 apart, take the same turn; a value that is not finite moves nothing.  In float16 the bf16 case above
 // takes 275 us with it, 261 without, the f32 one 41 and 38.)
-constexpr int kLift = 60;                                    // at first: 2^60 times what float16 operands make of dP stays a 32-bit number
+constexpr int kFirst = 60;                                   // at first: 2^60 times 2^15 P times what float16 operands make of dP stays a 32-bit number
 template <int N> __device__ __forceinline__ void fit(f32x16& x, int& lift, f32x16 (&acc)[N]) {
   float top = 0.f;
 #pragma unroll
@@ -70,8 +72,8 @@ template <int N> __device__ __forceinline__ void fit(f32x16& x, int& lift, f32x1
   }
 }
 
-// 32 RG query rows of one head; KS key groups of waves, as in the forward kernel.  Leaves delta and lse log2 e of its rows for the other
-// kernel: delta [2][heads][rows_q].
+// 32 RG query rows of one head; KS key groups of waves, as in the forward kernel.  Leaves delta and lse log2 e of its rows (less the lift of their
+// weights) for the other kernel: delta [2][heads][rows_q].
 template <typename T, int DP, int RG, int KS>
 __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_kernel(const SeqGradArgs ga, const int tiles) {
   typedef SeqTile<T, DP> L;
@@ -171,9 +173,9 @@ __global__ void __launch_bounds__(64 * RG * KS, sizeof(T) == 2 ? 2 : 1) seq_dq_k
     sum = seq_pair_sum(sum);
     delta = limit <= kFew ? sum : delta;
   }
-  if (live && g == 0 && kg == 0) { ga.delta[place] = delta; ga.delta[(long long)a.heads * a.rows_q + place] = lse2; }
+  if (live && g == 0 && kg == 0) { ga.delta[place] = delta; ga.delta[(long long)a.heads * a.rows_q + place] = lse2 - Weight<T>::kLift; }
   constexpr bool kFit = __is_same(T, _Float16);
-  int lift = kFit ? kLift : 0;
+  int lift = kFit ? kFirst : 0;
   int k0 = (kg - KS) * BN, stage = 0;                        // (the first turn only fetches)
   for (int kt = -step; kt < some; kt += step, k0 += step, stage ^= kStage) {
     seq_dma_wait();
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
   // ---- one tile of rows: the two products, the weights and their gradients, what they add to dV and dK ----------------------------------------
   f32x16 s, p;
   constexpr bool kFit = __is_same(T, _Float16);
-  int lift = kFit ? kLift : 0;
+  int lift = kFit ? kFirst : 0;
   SeqReads<T, DP> reads;
   reads.set(lane);
   auto products = [&](unsigned tile) {
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dk[d][i] = __builtin_amdgcn_ldexpf(dk[d][i], -lift);
+      for (int i = 0; i < 16; ++i) { dk[d][i] = __builtin_amdgcn_ldexpf(dk[d][i], -lift - (int)Weight<T>::kLift); dv[d][i] *= 1.f / Weight<T>::kTimes; }
   }
   if (HG > 1) {                                              // the row groups' sums, in their order: dK, then dV through the same buffer
     constexpr int N = (DP / 32) * 16;
