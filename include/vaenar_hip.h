@@ -258,7 +258,8 @@ int vnr_op_positional_encoding(vnr_handle h, int T, int dim, float step, float *
  * maxima, sums and accumulators are 32 bits.  head_dim: a multiple of 8, at most 128.  Matrices: 16-byte aligned, row strides a multiple
  * of 16 bytes.  scale > 0.  Outputs must not overlap inputs.  Rows outside d_cu[0] .. d_cu[batch] - 1 are neither read nor written, and a
  * masked or absent key contributes nothing whatever it holds (infinities and NaN included) -- see vnr_op_packed_attention_grad for its
- * exception.  Starts that run backwards or leave the tensor make a sequence empty; nothing outside a tensor is touched.  Refused calls
+ * exception.  Starts that run backwards make that sequence empty, starts outside the tensor count as its border -- for every operator alike --;
+ * rows that more than one sequence then claims hold no defined values, nothing outside a tensor is touched.  Refused calls
  * return VNR_ERR_ARG with a message and launch nothing.  All calls are asynchronous on the handle's stream, which is not any other
  * library's: memory that another stream writes has to be complete before the call. */
 enum { VNR_F32 = 0, VNR_F16 = 1, VNR_BF16 = 2 };

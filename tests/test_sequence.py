@@ -1020,3 +1020,52 @@ def test_small_weights_of_float16_reach_dv(eng, dim):
     out, lse = sequence.packed_attention(eng, *d, cq, ck, causal=False, scale=1.0)
     dv = sequence.packed_attention_grad(eng, eng.to_device(do), *d, out, lse, cq, ck, causal=False, scale=1.0)[2]
     close(dv.numpy()[1:], [x[1:] for x in want], "dv", "f16")
+
+
+BROKEN = [
+    # starts of 50 rows, and which sequence owns each range of them (first row, rows behind the last, place of the first row in its sequence)
+    ([0, 50, 20], [(0, 0, 50)]),                                  # 50..20 is empty, 0..50 is not
+    ([-7, 12, 30], [(0, 0, 12), (1, 12, 30)]),                    # a start in front of the tensor is its first row
+    ([5, 5, 1000], [(1, 5, 50)]),                                 # an end behind it its last
+    ([30, 10, 25], [(1, 10, 25)]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("bound", [200, 3000])                    # one piece of the keys, and several that are joined
+@pytest.mark.parametrize("case", BROKEN, ids=[str(i) for i in range(len(BROKEN))])
+def test_cache_calls_with_broken_starts(eng, case, bound, kind):
+    """Append and attention agree on who owns which row, whether the keys are cut or not: a broken start takes rows from its own sequences only, and rows
+    that are nobody's stay as they were."""
+    cu, owned = case
+    H, G, D, P, u = 4, 2, 64, 16, KINDS[kind][1]
+    r = np.random.default_rng(bound)
+    ctx = [70, 110]
+    table, pages = layout(r, [bound, bound], P)
+    q, k, v = normal(r, kind, 50, H, D), normal(r, kind, 50, G, D), normal(r, kind, 50, G, D)
+    kc, vc = normal(r, kind, pages, G, P, D), normal(r, kind, pages, G, P, D)
+    cache = sequence.PagedCache(eng, eng.to_device(kc), eng.to_device(vc))
+    dcu, dctx, dt = eng.to_device(np.int32(cu)), eng.to_device(np.int32(ctx)), eng.to_device(table)
+    mark = store(np.full(1, 7.0, np.float32), kind)[0]
+    qo, out = (eng.to_device(np.full(q.shape, mark, q.dtype)) for _ in range(2))
+    lse = eng.to_device(np.full((H, 50), 7.0, np.float32))
+    cache.append(eng.to_device(k), eng.to_device(v), dcu, dctx, dt, q=eng.to_device(q), q_out=qo)
+    wk, wv = kc.copy(), vc.copy()
+    nobody = np.ones(50, bool)
+    for b, i, j in owned:
+        nobody[i:j] = False
+        for t in range(i, j):
+            p = ctx[b] + t - i
+            wk[table[b, p // P], :, p % P], wv[table[b, p // P], :, p % P] = k[t], v[t]
+    assert (cache.k.numpy() == wk).all() and (cache.v.numpy() == wv).all()
+    gq = qo.numpy()
+    assert (gq[~nobody] == q[~nobody]).all() and (gq[nobody] == mark).all()
+    cache.attend(eng.to_device(q), dcu, dctx, dt, 50, bound, out=out, lse=lse)
+    got, gl = out.numpy(), lse.numpy()
+    for b, i, j in owned:
+        held = [x[table[b]].transpose(0, 2, 1, 3).reshape(-1, G, D)[:ctx[b] + j - i] for x in (wk, wv)]
+        want = definition(value(q[i:j]), value(held[0]), value(held[1]), starts([j - i]), starts([ctx[b] + j - i]), True, D ** -0.5, u, first=[ctx[b]])
+        close(got[i:j], want["out"], "out", kind)
+        close(gl[:, i:j], want["lse"], "lse")
+    assert (got[nobody] == mark).all() and (gl[:, nobody] == 7).all()

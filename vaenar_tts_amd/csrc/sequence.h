@@ -272,8 +272,29 @@ __device__ __forceinline__ int seq_scalar(const int32_t* p) {
   return *(const __attribute__((address_space(4))) int*)(unsigned long long)p;
 }
 
-// The sequence and the tile in it that a workgroup's tile index names: every sequence of n rows has ceil(n * mult / rows) tiles.  Starts that
-// run backwards or leave the tensor are clamped: such a sequence is empty, nothing outside the tensor is touched.  `other` (or null): x0 =
+// A sequence's rows, by one rule for every operator: its starts are clamped to the tensor, and one whose end lies in front of its start is empty
+__device__ __forceinline__ void seq_clamp(int s, int e, int total, int& start, int& n) {
+  s = s < 0 ? 0 : (s > total ? total : s);
+  e = e < s ? s : (e > total ? total : e);
+  start = s; n = e - s;
+}
+// The sequence that owns row `token` (the first where starts overlap; -1: none) and its first row: 64 sequences a look
+__device__ __forceinline__ int seq_owner(const int32_t* cu, int batch, int total, int token, int& start) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    int s = 0, n = 0;
+    if (b0 + lane < batch) seq_clamp(cu[b0 + lane], cu[b0 + lane + 1], total, s, n);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(s <= token && token < s + n);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      start = __builtin_amdgcn_readlane(s, src);
+      return b0 + src;
+    }
+  }
+  return -1;
+}
+// The sequence and the tile in it that a workgroup's tile index names: every sequence of n rows has ceil(n * mult / rows) tiles.  Nothing
+// outside the tensor is touched, whatever the starts are.  `other` (or null): x0 =
 // other[b], x1 = other[b + two], fetched along with the starts.  Where the launch has more workgroups than the chip
 // holds at once, up to 64 sequences are gone through from the longest (rows, or rows + x0 where x0 counts keys in front of them: `two` 0) to
 // the shortest: it ends with its short tasks (eight chunks of up to 512 rows over up to 6000 keys: 223 -> 187 us; about 1 us of a small launch).
@@ -288,9 +309,8 @@ __device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total
       s = cu[b]; e = cu[b + 1];
       if (other) { x0 = other[b]; x1 = other[b + two]; }
     }
-    s = s < 0 ? 0 : (s > total ? total : s);
-    e = e < s ? s : (e > total ? total : e);
-    int n = e - s;
+    int n;
+    seq_clamp(s, e, total, s, n);
     int t = (int)(((long long)n * mult + rows - 1) / rows);
     if (gridDim.x > 512 && batch > 1 && batch <= 64) {       // ranks, then everything to the lane of its rank
       const int key = b < batch ? n + (two ? 0 : x0 < 1 << 30 ? x0 : 1 << 30) : -1;
@@ -315,11 +335,6 @@ __device__ __forceinline__ bool seq_find(const int32_t* cu, int batch, int total
     before += __builtin_amdgcn_readlane(x, 63);
   }
   return false;
-}
-__device__ __forceinline__ void seq_clamp(int s, int e, int total, int& start, int& n) {
-  s = s < 0 ? 0 : (s > total ? total : s);
-  e = e < s ? s : (e > total ? total : e);
-  start = s; n = e - s;
 }
 // workgroup -> task: the hardware deals workgroups to the 8 XCDs in turn, the tasks of one XCD are to be neighbours (the same keys in its L2)
 __device__ __forceinline__ int seq_task(int id, int n) {

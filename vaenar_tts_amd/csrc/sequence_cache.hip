@@ -32,15 +32,9 @@ template <typename T> struct Turn {
 template <typename T>
 __global__ void __launch_bounds__(256) seq_append_kernel(const SeqAppendArgs a) {
   typedef typename SeqVec<T>::v8 v8;
-  const int token = blockIdx.x, lane = threadIdx.x & 63;
-  // the token's sequence: 64 sequences a look
-  int b = -1, start = 0;
-  for (int b0 = 0; b0 < a.batch && b < 0; b0 += 64) {
-    int s = 0, e = 0;
-    if (b0 + lane < a.batch) { s = a.cu[b0 + lane]; e = a.cu[b0 + lane + 1]; }
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(s >= 0 && s <= token && token < e);
-    if (hit) { const int src = __builtin_ctzll(hit); b = __builtin_amdgcn_readfirstlane(b0 + src); start = __builtin_amdgcn_readfirstlane(__shfl(s, src, 64)); }
-  }
+  const int token = blockIdx.x;
+  int start = 0;
+  const int b = seq_owner(a.cu, a.batch, a.rows, token, start);
   if (b < 0) return;                                         // a row outside the sequences: nothing is read or written
   int pos = a.ctx[b];
   pos = (pos < 0 ? 0 : pos);

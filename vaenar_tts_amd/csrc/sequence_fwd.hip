@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqArgs a) {
   const long long pr = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), n = (long long)a.rows_q * a.heads;
   if (pr >= n) return;
   const int token = (int)(pr / a.heads), head = (int)(pr - (long long)token * a.heads);
-  if (token < a.cu_q[0] || token >= a.cu_q[a.batch]) return;         // rows outside the sequences stay as they were
+  int start;
+  if (seq_owner(a.cu_q, a.batch, a.rows_q, token, start) < 0) return;          // rows outside the sequences stay as they were
   join_row<T>(a, pr, n, token, head, threadIdx.x & 63);
 }
 
