@@ -1069,3 +1069,21 @@ def test_cache_calls_with_broken_starts(eng, case, bound, kind):
         close(got[i:j], want["out"], "out", kind)
         close(gl[:, i:j], want["lse"], "lse")
     assert (got[nobody] == mark).all() and (gl[:, nobody] == 7).all()
+
+
+def test_library_refusals_of_more_rows_than_a_launch_holds():
+    """Before anything is launched -- a gradient's second kernel included -- and as an error of the arguments."""
+    far = dict(heads=4096, kv_heads=4096, ldq=4096 * 64, ldk=4096 * 64, ldv=4096 * 64, ldo=4096 * 64)
+    most = (1 << 31) - 1
+    grad = _lib.vnr_packed_attention_grad(d_dout=4096, lddo=4096 * 64, d_dq=4096, d_dk=4096, d_dv=4096, lddq=4096 * 64, lddk=4096 * 64, lddv=4096 * 64)
+    for kw in (dict(rows_q=most), dict(rows_q=1 << 20)):
+        assert "launch" in refused("vnr_op_packed_attention", packed_desc(**far, **kw)), kw
+        assert "launch" in refused("vnr_op_packed_attention_grad", packed_desc(d_lse=64, **far, **kw), grad), kw
+    for kw in (dict(rows_k=most), dict(rows_k=1 << 20), dict(rows_q=0, rows_k=most)):
+        assert "null handle" in refused("vnr_op_packed_attention", packed_desc(**far, **kw)), kw      # keys do not make the forward's launch
+        assert "launch" in refused("vnr_op_packed_attention_grad", packed_desc(d_lse=64, **far, **kw), grad), kw
+    cache = _lib.vnr_kv_cache(dtype=1, kv_heads=2, head_dim=64, pages=8, page_size=16, d_k=4096, d_v=4096)
+    att = dict(batch=2, heads=4096, rows=most, d_cu=64, d_context=64, d_table=64, table_width=3, max_new=4, max_context=40, scale=0.125, d_q=4096, ldq=4096 * 64,
+               d_out=4096, ldo=4096 * 64, d_lse=None)
+    assert "launch" in refused("vnr_op_paged_attention", cache, _lib.vnr_paged_attention_desc(**att))
+    assert "launch" in refused("vnr_op_paged_attention", cache, _lib.vnr_paged_attention_desc(**{**att, "rows": 1 << 20}))

@@ -26,6 +26,8 @@ struct SeqArgs {
 // the launch that seq_plan() chose for these sizes: how many of a workgroup's four waves stand side by side along the rows (the others: along the keys)
 struct SeqPlan { int row_waves = 4, splits = 1, chunk = 0; };
 SeqPlan seq_plan(const SeqArgs& a, int compute_units);
+bool seq_fwd_fits(const SeqArgs& a, const SeqPlan& p);       // do the grids hold that many rows and heads? (a launch has at most 2^32 - 1 threads)
+bool seq_grad_fits(const SeqArgs& a);
 hipError_t launch_seq_fwd(const SeqArgs& a, const SeqPlan& p, hipStream_t s);
 hipError_t launch_seq_join(const SeqArgs& a, hipStream_t s);
 

@@ -443,16 +443,23 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
     }
 }
 
+// tiles of `rows` rows, at most: every sequence ends inside one
+long long tiles_of(int total, int batch, int rows) { return total / rows + (batch < total ? batch : total); }
+// Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 256 / 294 us
+// with four / two), two of them and twice the workgroups a unit where they pass few (the f32 case 124 / 113); rows of 512 bytes leave room for two
+int row_groups(const SeqArgs& f) {
+  const long long turns = (long long)f.rows_q / f.batch * (f.heads / f.kv_heads) / 32;
+  return (f.dtype == SEQ_F32 ? 4 : 2) * (f.dim <= 64 ? 64 : 128) <= 256 && turns >= 32 ? 4 : 2;
+}
+
 template <typename T, int DP, int RG, int KS> hipError_t grad_q(const SeqGradArgs& a, hipStream_t s) {
   static int done[kMaxDevices];
   constexpr int BN = RG == 4 ? 64 : 32, tiles_lds = KS * 4 * BN * SeqTile<T, DP>::kRow, join = (KS - 1) * RG * (DP / 32) * 16 * 256, lds = tiles_lds > join ? tiles_lds : join;
   static_assert(lds <= 160 * 1024, "LDS");
   opt_in_dynamic_lds((const void*)seq_dq_kernel<T, DP, RG, KS>, lds, done);
   const SeqArgs& f = a.f;
-  const int tiles = f.rows_q / (32 * RG) + (f.batch < f.rows_q ? f.batch : f.rows_q);
-  const long long grid = (long long)tiles * f.heads;
-  if (grid >= 1 << 24) return hipErrorInvalidValue;           // (2^32 threads)
-  vnr_launch(seq_dq_kernel<T, DP, RG, KS>, dim3((unsigned)grid), dim3(64 * RG * KS), lds, s, a, tiles);
+  const int tiles = (int)tiles_of(f.rows_q, f.batch, 32 * RG);
+  vnr_launch(seq_dq_kernel<T, DP, RG, KS>, dim3((unsigned)tiles * f.heads), dim3(64 * RG * KS), lds, s, a, tiles);
   return hipGetLastError();
 }
 template <typename T, int DP, int KG, int HG> hipError_t grad_kv(const SeqGradArgs& a, hipStream_t s) {
@@ -461,10 +468,8 @@ template <typename T, int DP, int KG, int HG> hipError_t grad_kv(const SeqGradAr
   static_assert(lds <= 160 * 1024, "LDS");
   opt_in_dynamic_lds((const void*)seq_dkv_kernel<T, DP, KG, HG>, lds, done);
   const SeqArgs& f = a.f;
-  const int tiles = f.rows_k / (32 * KG) + (f.batch < f.rows_k ? f.batch : f.rows_k);
-  const long long grid = (long long)tiles * f.kv_heads;
-  if (grid >= (1LL << 32) / (64 * KG * HG)) return hipErrorInvalidValue;
-  vnr_launch(seq_dkv_kernel<T, DP, KG, HG>, dim3((unsigned)grid), dim3(64 * KG * HG), lds, s, a, tiles);
+  const int tiles = (int)tiles_of(f.rows_k, f.batch, 32 * KG);
+  vnr_launch(seq_dkv_kernel<T, DP, KG, HG>, dim3((unsigned)tiles * f.kv_heads), dim3(64 * KG * HG), lds, s, a, tiles);
   return hipGetLastError();
 }
 template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, int cus, hipStream_t s) {
@@ -472,18 +477,19 @@ template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, int cus, hip
   const SeqArgs& f = a.f;
   // 128 query rows a workgroup where that makes two for each compute unit, else 64 (32 utterances of up to 400 rows, 4 heads, f32: both kernels
   // 135 / 113 us with 128 / 64; 4 sequences of up to 2048, 32 heads of 128, bf16: 256 / 269)
-  const long long wgs = ((long long)f.rows_q / 128 + (f.batch < f.rows_q ? f.batch : f.rows_q)) * f.heads;
+  const long long wgs = tiles_of(f.rows_q, f.batch, 128) * f.heads;
   if (f.rows_q > 0) e = wgs >= 2LL * cus ? grad_q<T, DP, 4, 1>(a, s) : grad_q<T, DP, 2, 2>(a, s);
   if (e != hipSuccess || f.rows_k == 0) return e;
-  // Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 256 / 294 us
-  // with four / two), two of them and twice the workgroups a unit where they pass few (the f32 case 124 / 113); rows of 512 bytes leave room for two
-  const long long turns = (long long)f.rows_q / f.batch * (f.heads / f.kv_heads) / 32;
-  if (sizeof(T) * DP <= 256 && turns >= 32) return grad_kv<T, DP, 2, (sizeof(T) * DP > 256 ? 2 : 4)>(a, s);
+  if (row_groups(f) == 4) return grad_kv<T, DP, 2, (sizeof(T) * DP > 256 ? 2 : 4)>(a, s);
   return grad_kv<T, DP, 2, 2>(a, s);
 }
 template <typename T> hipError_t grad(const SeqGradArgs& a, int cus, hipStream_t s) { return a.f.dim <= 64 ? grad<T, 64>(a, cus, s) : grad<T, 128>(a, cus, s); }
 }  // namespace
 
+// (256 threads a workgroup of dQ, of 128 rows at least where there are more than the chip holds; 64 keys and 128 threads a row group of dK and dV)
+bool seq_grad_fits(const SeqArgs& f) {
+  return tiles_of(f.rows_q, f.batch, 128) * f.heads < 1LL << 24 && tiles_of(f.rows_k, f.batch, 64) * f.kv_heads < (1LL << 32) / (128 * row_groups(f));
+}
 hipError_t launch_seq_grad(const SeqGradArgs& a, int cus, hipStream_t s) {
   if (a.f.dtype == SEQ_F32) return grad<float>(a, cus, s);
   if (a.f.dtype == SEQ_F16) return grad<_Float16>(a, cus, s);

@@ -415,10 +415,14 @@ __global__ void __launch_bounds__(256) seq_join_kernel(const SeqArgs a) {
   join_row<T>(a, pr, n, token, head, threadIdx.x & 63);
 }
 
-int tiles_of(const SeqArgs& a, int mult, int bm) {           // at most: every sequence ends inside a tile
-  const long long r = (long long)a.rows_q * mult;
-  return (int)(r / bm) + (a.batch < a.rows_q ? a.batch : a.rows_q);
+long long tiles_of(const SeqArgs& a, int mult, int bm) {     // at most: every sequence ends inside a tile
+  return (long long)a.rows_q * mult / bm + (a.batch < a.rows_q ? a.batch : a.rows_q);
 }
+// workgroups of `row_waves` x 32 rows, and of four waves at most
+long long grid_of(const SeqArgs& a, int row_waves, int splits) {
+  return a.table ? tiles_of(a, a.heads / a.kv_heads, 32 * row_waves) * a.kv_heads * splits : tiles_of(a, 1, 32 * row_waves) * a.heads;
+}
+constexpr long long kMostWorkgroups = (1 << 24) - 1;         // of 256 threads
 
 template <typename T, int DP, bool PAGED, int RG, int KS>
 hipError_t fwd(const SeqArgs& a, hipStream_t s) {
@@ -427,10 +431,8 @@ hipError_t fwd(const SeqArgs& a, hipStream_t s) {
   constexpr int lds = F::kLds > F::kJoin ? F::kLds : F::kJoin;
   static_assert(lds <= 160 * 1024, "LDS");
   opt_in_dynamic_lds((const void*)seq_fwd_kernel<T, DP, PAGED, RG, KS>, lds, done);
-  const int mult = PAGED ? a.heads / a.kv_heads : 1, tiles = tiles_of(a, mult, F::BM);
-  const long long grid = (long long)tiles * (PAGED ? (long long)a.kv_heads * a.splits : a.heads);
-  if (grid >= 1 << 24) return hipErrorInvalidValue;           // (2^32 threads)
-  vnr_launch(seq_fwd_kernel<T, DP, PAGED, RG, KS>, dim3((unsigned)grid), dim3(64 * RG * KS), lds, s, a, tiles);
+  const int tiles = (int)tiles_of(a, PAGED ? a.heads / a.kv_heads : 1, F::BM);
+  vnr_launch(seq_fwd_kernel<T, DP, PAGED, RG, KS>, dim3((unsigned)grid_of(a, RG, a.splits)), dim3(64 * RG * KS), lds, s, a, tiles);
   return hipGetLastError();
 }
 template <typename T, int DP, bool PAGED>
@@ -443,6 +445,7 @@ template <typename T> hipError_t fwd(const SeqArgs& a, const SeqPlan& p, hipStre
   if (a.dim <= 64) return a.table ? fwd<T, 64, true>(a, p, s) : fwd<T, 64, false>(a, p, s);
   return a.table ? fwd<T, 128, true>(a, p, s) : fwd<T, 128, false>(a, p, s);
 }
+long long join_grid(const SeqArgs& a) { return ((long long)a.rows_q * a.heads + 3) / 4; }
 }  // namespace
 
 // Rows a workgroup.  Packed: 128 (every key tile is read once for them) where that makes two workgroups for each compute unit; else 64, else 32
@@ -455,11 +458,11 @@ SeqPlan seq_plan(const SeqArgs& a, int cus) {
   SeqPlan p;
   const int group = a.heads / a.kv_heads;
   if (!a.table) {
-    while (p.row_waves > 1 && (long long)tiles_of(a, 1, 32 * p.row_waves) * a.heads < 2LL * cus) p.row_waves /= 2;
+    while (p.row_waves > 1 && grid_of(a, p.row_waves, 1) < 2LL * cus) p.row_waves /= 2;
     return p;
   }
   p.row_waves = (long long)a.max_new * group > 64 ? 4 : 2;
-  const long long wgs = (long long)tiles_of(a, group, 32 * p.row_waves) * a.kv_heads;
+  const long long wgs = grid_of(a, p.row_waves, 1);
   long long want = wgs > 0 ? (2LL * cus + wgs - 1) / wgs : 1;
   const long long most = (a.max_context + 255) / 256;
   if (want > most) want = most;
@@ -470,14 +473,16 @@ SeqPlan seq_plan(const SeqArgs& a, int cus) {
   return p;
 }
 
+bool seq_fwd_fits(const SeqArgs& a, const SeqPlan& p) {
+  return grid_of(a, p.row_waves, p.splits) <= kMostWorkgroups && (p.splits == 1 || join_grid(a) <= kMostWorkgroups);
+}
 hipError_t launch_seq_fwd(const SeqArgs& a, const SeqPlan& p, hipStream_t s) {
   if (a.dtype == SEQ_F32) return fwd<float>(a, p, s);
   if (a.dtype == SEQ_F16) return fwd<_Float16>(a, p, s);
   return fwd<sq_bf16>(a, p, s);
 }
 hipError_t launch_seq_join(const SeqArgs& a, hipStream_t s) {
-  const long long n = (long long)a.rows_q * a.heads, grid = (n + 3) / 4;
-  if (grid >= 1 << 24) return hipErrorInvalidValue;           // (2^32 threads)
+  const long long grid = join_grid(a);
   if (a.dtype == SEQ_F32) vnr_launch(seq_join_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, a);
   else if (a.dtype == SEQ_F16) vnr_launch(seq_join_kernel<_Float16>, dim3((unsigned)grid), dim3(256), 0, s, a);
   else vnr_launch(seq_join_kernel<sq_bf16>, dim3((unsigned)grid), dim3(256), 0, s, a);
