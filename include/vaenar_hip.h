@@ -261,7 +261,8 @@ int vnr_op_positional_encoding(vnr_handle h, int T, int dim, float step, float *
  * exception.  Starts that run backwards make that sequence empty, starts outside the tensor count as its border -- for every operator alike --;
  * rows that more than one sequence then claims hold no defined values, nothing outside a tensor is touched.  Refused calls
  * return VNR_ERR_ARG with a message and launch nothing.  All calls are asynchronous on the handle's stream, which is not any other
- * library's: memory that another stream writes has to be complete before the call. */
+ * library's: memory that another stream writes has to be complete before the call.  They look for no range word and raise none: one that
+ * took results which VNR_ERR_RANGE voids is to be issued again like any other, over the same contents of d_context and d_table. */
 enum { VNR_F32 = 0, VNR_F16 = 1, VNR_BF16 = 2 };
 typedef struct vnr_packed_attention_desc {
   int32_t dtype, batch, heads, kv_heads, head_dim;

@@ -1087,3 +1087,55 @@ def test_library_refusals_of_more_rows_than_a_launch_holds():
                d_out=4096, ldo=4096 * 64, d_lse=None)
     assert "launch" in refused("vnr_op_paged_attention", cache, _lib.vnr_paged_attention_desc(**att))
     assert "launch" in refused("vnr_op_paged_attention", cache, _lib.vnr_paged_attention_desc(**{**att, "rows": 1 << 20}))
+
+
+class Script:
+    """The library as far as the engine's log needs it: notes the calls in order; the checkpoint that follows `trip` finds the range word raised once."""
+
+    def __init__(self, trip):
+        self.trip, self.raised, self.calls = trip, False, []
+
+    def vnr_last_error(self, handle):
+        return b"range"
+
+    def __getattr__(self, name):
+        if not name.startswith("vnr_"):
+            raise AttributeError(name)
+
+        def fn(handle, *args):
+            self.calls.append(name)
+            if name == self.trip:
+                self.raised, self.trip = True, None
+            if name in ("vnr_synchronize", "vnr_memcpy_d2h", "vnr_memcpy_h2d") and self.raised:
+                self.raised = False
+                return _lib.VNR_ERR_RANGE
+            return 0
+        return fn
+
+
+def test_cache_calls_run_once_whatever_the_range_sentinel_finds(monkeypatch):
+    """A module call whose results a raised range word voids is issued again at the next checkpoint.  Calls of this file stand behind such a checkpoint and
+    are not issued again themselves: another library may own their arrays and may have moved the context or the table on by then."""
+    lib = Script("vnr_prior_sample")
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    e = _lib.Engine.__new__(_lib.Engine)
+    e.lib, e.handle, e._log, e._log_cap, e._training_mode, e.range_replays = lib, 1, [], 256, False, 0
+    e._pool, e._pool_bytes, e._pool_cap = {}, 0, 1 << 30
+    array = lambda shape, kind=np.float16: _lib.DeviceArray(e, shape, kind, ptr=4096, owner=lib)
+    q, k, cu, cu1, ctx, table = array((6, 4, 64)), array((6, 2, 64)), array((3,), np.int32), array((3,), np.int32), array((2,), np.int32), array((2, 3), np.int32)
+    cache = sequence.PagedCache(e, array((4, 2, 16, 64)), array((4, 2, 16, 64)))
+    rot, lse = array((48, 64), np.float32), array((4, 6), np.float32)
+    e.call("vnr_prior_sample")
+    cache.append(k, k, cu, ctx, table, rotation=rot, q=q, q_out=q)
+    cache.attend(q, cu, ctx, table, 1, 40, out=q)
+    sequence.packed_attention(e, q, k, k, cu, out=q, lse=lse)
+    sequence.packed_attention_grad(e, q, q, k, k, q, lse, cu, dq=q, dk=k, dv=k)
+    e.synchronize()
+    assert lib.calls == ["vnr_prior_sample", "vnr_synchronize", "vnr_prior_sample", "vnr_synchronize", "vnr_op_kv_append", "vnr_op_paged_attention",
+                         "vnr_op_packed_attention", "vnr_op_packed_attention_grad", "vnr_synchronize"]
+    # a loop of them keeps no log, and the host does not wait for the device in it
+    lib.calls.clear()
+    for _ in range(300):
+        cache.attend(q, cu, ctx, table, 1, 40, out=q)
+    assert lib.calls == ["vnr_op_paged_attention"] * 300 and not e._log
+    e.handle = None

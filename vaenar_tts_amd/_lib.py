@@ -363,6 +363,13 @@ class Engine:
             if len(self._log) >= self._log_cap:
                 self.synchronize()
 
+    def call_once(self, name, *args):
+        """An entry point that is never issued again: its arrays may be another library's, which may have freed or rewritten them by the time
+        of a replay.  What is pending is settled first (a synchronisation, and the replay if the word is raised); the call itself is not recorded."""
+        if self._pending():
+            self.synchronize()
+        self.call(name, *args, record=False)
+
     def _pending(self):
         """True while a compute call waits for its checkpoint (option settings alone do not count)."""
         return any(name != "vnr_set_option" for name, _ in self._log)

@@ -7,6 +7,9 @@ in elements) let q, k and v be column blocks of one projection: pass a view of t
 
 The prompt of a batch goes through ``packed_attention`` and ``PagedCache.append``; every later chunk of rows -- one row a sequence in a
 decoding step -- through ``append`` and ``attend``.  ``packed_attention_grad`` is the backward pass of ``packed_attention``.
+
+Every call runs once (``Engine.call_once``): one that follows calls of the model waits until their results are known to hold, and none is
+issued again when the range word is raised later.  Context, table and starts may therefore be rewritten in place between calls.
 """
 import ctypes as C
 
@@ -86,7 +89,7 @@ def packed_attention(engine, q, k, v, cu_q, cu_k=None, causal=True, scale=None, 
     if lse is None:
         lse = engine.empty((q.shape[1], q.shape[0]))
     d = _packed_desc("packed_attention", q, k, v, cu_q, cu_q if cu_k is None else cu_k, causal, scale, out, lse, ldq, ldk, ldv, ldo)
-    engine.call("vnr_op_packed_attention", C.byref(d))
+    engine.call_once("vnr_op_packed_attention", C.byref(d))
     return out, lse
 
 
@@ -103,14 +106,14 @@ def packed_attention_grad(engine, dout, q, k, v, out, lse, cu_q, cu_k=None, caus
         _shape(who, name, a, like.shape)
     wq, wk = d.heads * d.head_dim, d.kv_heads * d.head_dim
     g = vnr_packed_attention_grad(dout.ptr, lddout or wq, dq.ptr, dk.ptr, dv.ptr, lddq or wq, lddk or wk, lddv or wk)
-    engine.call("vnr_op_packed_attention_grad", C.byref(d), C.byref(g))
+    engine.call_once("vnr_op_packed_attention_grad", C.byref(d), C.byref(g))
     return dq, dk, dv
 
 
 def rotation_table(engine, positions, rot_dim, base=10000.0):
     """float32 [positions, rot_dim]: cosines, then sines, of position / base ** (2 c / rot_dim)."""
     t = engine.empty((int(positions), int(rot_dim)))
-    engine.call("vnr_op_rotation_table", int(positions), int(rot_dim), float(base), t.ptr)
+    engine.call_once("vnr_op_rotation_table", int(positions), int(rot_dim), float(base), t.ptr)
     return t
 
 
@@ -126,7 +129,6 @@ class PagedCache:
         self.engine, self.k, self.v = engine, k, v
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self._kind, self._row = k.dtype, (self.kv_heads, self.head_dim)
-        # fixed for the cache's life: the calls that a range trip makes the engine issue again point to it
         self._desc = vnr_kv_cache(_code(who, k, v), self.kv_heads, self.head_dim, self.pages, self.page_size, k.ptr, v.ptr)
         self._ref = C.byref(self._desc)
 
@@ -175,7 +177,7 @@ class PagedCache:
         d = vnr_kv_append_desc(batch, heads, rows, cu.ptr, context.ptr, table.ptr, table.shape[1], k.ptr, v.ptr, ldk or wk, ldv or wk,
                                None if q is None else q.ptr, None if q is None else q_out.ptr, ldq or wq, ldqo or wq, rot[0], rot[1], rot[2],
                                1 if interleaved else 0)
-        self.engine.call("vnr_op_kv_append", self._ref, C.byref(d))
+        self.engine.call_once("vnr_op_kv_append", self._ref, C.byref(d))
         return q_out
 
     def attend(self, q, cu, context, table, max_new, max_context, scale=None, out=None, lse=None, ldq=None, ldo=None):
@@ -198,5 +200,5 @@ class PagedCache:
         d = vnr_paged_attention_desc(batch, heads, rows, cu.ptr, context.ptr, table.ptr, table.shape[1], int(max_new), int(max_context),
                                      self.head_dim ** -0.5 if scale is None else scale, q.ptr, ldq or wq, out.ptr, ldo or wq,
                                      None if lse is None else lse.ptr)
-        self.engine.call("vnr_op_paged_attention", self._ref, C.byref(d))
+        self.engine.call_once("vnr_op_paged_attention", self._ref, C.byref(d))
         return out
