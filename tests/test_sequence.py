@@ -1139,3 +1139,37 @@ def test_cache_calls_run_once_whatever_the_range_sentinel_finds(monkeypatch):
         cache.attend(q, cu, ctx, table, 1, 40, out=q)
     assert lib.calls == ["vnr_op_paged_attention"] * 300 and not e._log
     e.handle = None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [1, 160])
+@pytest.mark.parametrize("size", [10, 12, 14])
+def test_logits_far_beyond_their_own_steps(eng, size, heads, kind):
+    """Logits of up to 2^29, whose neighbours in 32 bits are tens apart: weights stay weights (the bound that is taken off a row's logits may not be rounded
+    below them), and a row whose largest logit leaves the others far behind gets that key's value."""
+    r = np.random.default_rng(size)
+    n, D, P = 300, 128, 16
+    q, k = (store(r.standard_normal((n, h, D)).clip(-3.9, 3.9) * 2.0 ** size, kind) for h in (heads, 1))
+    v = normal(r, kind, n, 1, D)
+    c, scale = starts([n]), np.float64(np.float32(D ** -0.5))
+    dq, dk, dv, dc = (eng.to_device(x) for x in (q, k, v, c))
+    out, lse = sequence.packed_attention(eng, dq, dk, dv, dc)
+    table, pages = layout(r, [n], P)
+    cache = sequence.PagedCache.empty(eng, pages, 1, P, D, KINDS[kind][0])
+    zero, dt = eng.to_device(np.int32([0])), eng.to_device(table)
+    cache.append(dk, dv, dc, zero, dt)
+    outs = [out, cache.attend(dq, dc, zero, dt, n, n), cache.attend(dq, dc, zero, dt, 1, 1 << 20)]
+    values = [value(x.numpy()) for x in outs]
+    K, V, u = value(k)[:, 0], value(v)[:, 0], KINDS[kind][1]
+    for h in (0, heads - 1):
+        x = np.where(np.tri(n, dtype=bool), value(q)[:, h] @ K.T * scale, -np.inf)
+        off = (D + 4) * H24 * scale * (np.abs(value(q)[:, h]) @ np.abs(K).T).max()      # of a logit in 32 bits
+        top = np.argmax(x, 1)
+        second = np.where(np.arange(n) == top[:, None], -np.inf, x).max(1)
+        clear = x.max(1) - second > 2 * off + 30
+        assert clear.mean() > 0.5
+        for got in values:
+            assert np.isfinite(got[:, h]).all()
+            assert (np.abs(got[clear, h] - V[top[clear]]) <= 2 * u * np.abs(V[top[clear]]) + n * 1e-12).all()
+    assert np.isfinite(lse.numpy()).all()

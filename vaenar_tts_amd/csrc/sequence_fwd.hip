@@ -109,13 +109,25 @@ struct Fwd {
   static_assert(kJoin <= 2 * KS * kStage, "the join lies where the tiles were");
 };
 
-// What is taken off a row's logits in units of log2, rounded once and the same wherever it is used: weights of different tiles stay in proportion
-template <typename T> __device__ __forceinline__ float bound(float m, float c) {
+// A row's weights under the bound m: exp2((s - sub) c + off).  What is taken off is the bound in units of log2, rounded once and the same wherever
+// it is used, so that weights of different tiles stay in proportion.  Beyond 2^16 that rounding is more than the weights can bear (from 2^27 on they
+// would be infinite or nothing), and logits and bound are subtracted in front of the product instead.
+struct Base { float sub, off; };
+template <typename T> __device__ __forceinline__ Base base_of(float m, float c) {
 #pragma clang fp contract(off)
-  return m * c - Weight<T>::kLift;
+  const float off = Weight<T>::kLift - m * c;
+  const bool far = __builtin_fabsf(off) > 65536.f, none = m == -__builtin_inff();
+  const Base b = {far && !none ? m : 0.f, none ? 0.f : (far ? Weight<T>::kLift : off)};
+  return b;
 }
-// the same without the weights' power of two (an exact sum: the bound lies on its own, coarser grid or is the exact difference)
-template <typename T> __device__ __forceinline__ float bare(float bound) { return bound + Weight<T>::kLift; }
+// weights under one base over those under another
+__device__ __forceinline__ float ratio(const Base& to, const Base& from, float c) { return __builtin_amdgcn_exp2f(__builtin_fmaf(from.sub - to.sub, c, to.off - from.off)); }
+// the logarithm of a row's sum `l` of weights: what the base's rounding left belongs to it
+template <typename T> __device__ __forceinline__ float log_sum(float m, float l, float scale) {
+  const float c = scale * kLog2e;
+  const Base b = base_of<T>(m, c);
+  return m * scale + (__logf(l * (1.f / Weight<T>::kTimes)) - kLn2 * __builtin_fmaf(m - b.sub, c, b.off - Weight<T>::kLift));
+}
 
 // The pieces of a row's keys joined by one wave, lanes along the channels
 template <typename T>
@@ -138,7 +150,8 @@ __device__ __forceinline__ void join_row(const SeqArgs& a, long long pr, long lo
       top = m;
 #pragma unroll
       for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-      f = l != 0.f ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+      const float c = a.scale * kLog2e;
+      f = l != 0.f ? ratio(base_of<T>(top, c), base_of<T>(m, c), c) : 0.f;
       sum = l * f;
 #pragma unroll
       for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s, 64);
@@ -150,12 +163,12 @@ __device__ __forceinline__ void join_row(const SeqArgs& a, long long pr, long lo
       if (s < a.splits && fs != 0.f) { x[0] += fs * p[i][0]; x[1] += fs * p[i][1]; }      // (an empty piece has left nothing)
     }
   }
-  const float inv = sum != 0.f ? 1.f / (sum * Weight<T>::kTimes) : 0.f;      // (the pieces' results carry the power of two)
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   if (2 * lane < a.dim) {
     T* op = (T*)a.out + token * a.ldo + (long long)head * a.dim + col;
     op[0] = (T)(x[0] * inv); op[1] = (T)(x[1] * inv);
   }
-  if (a.lse && lane == 0) a.lse[(long long)head * a.rows_q + token] = sum != 0.f ? top * kLn2 + __logf(sum) : -__builtin_inff();
+  if (a.lse && lane == 0) a.lse[(long long)head * a.rows_q + token] = sum != 0.f ? log_sum<T>(top, sum, a.scale) : -__builtin_inff();
 }
 
 template <typename T, int DP, bool PAGED, int RG, int KS>
@@ -232,7 +245,8 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m = -__builtin_inff(), l = 0.f;                      // running bound (of the raw products) and this lane's part of the row sum
   const float c = a.scale * kLog2e;
-  float mc = 0.f;                                            // bound(m, c)
+  Base w0 = {0.f, 0.f};                                      // base_of(m, c)
+  bool far = false;                                          // is any lane's beyond 2^16? (the same for the wave)
 
   char* base = smem + kg * 2 * F::kStage;
   const unsigned lds = seq_lds(base);
@@ -265,19 +279,26 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     mx = seq_pair_max(mx);
     if (__builtin_amdgcn_ballot_w64((mx - m) * c > Weight<T>::kSlack || (mx > m && m == -__builtin_inff()))) {
       const float m1 = fmaxf(m, mx);
-      const float b1 = m1 == -__builtin_inff() ? 0.f : bound<T>(m1, c);
-      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mc - b1);
-      m = m1; mc = b1;
+      const Base b = base_of<T>(m1, c);
+      const float f = m == -__builtin_inff() ? 0.f : ratio(b, w0, c);
+      m = m1; w0 = b;
+      far = __builtin_amdgcn_ballot_w64(b.sub != 0.f) != 0;
       l *= f;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= f;
     }
+    if (far) {
+#pragma unroll
+      for (int j = 0; j < F::NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[j][i] -= w0.sub;
+    }
 #pragma unroll
     for (int j = 0; j < F::NJ; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc)); l += s[j][i]; }
+      for (int i = 0; i < 16; ++i) { s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, w0.off)); l += s[j][i]; }
   };
   auto result = [&](unsigned tv) {
     const unsigned at = seq_at(tv, reads.col);
@@ -348,7 +369,8 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     for (int k = 0; kg == 0 && k < KS - 1; ++k) {
       const float* y = x + (k * RG + rg) * (N + 2) * 64;
       const float m2 = y[N * 64], l2 = y[(N + 1) * 64], m1 = fmaxf(m, m2);
-      const float mc = bound<T>(m1, c), f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound<T>(m, c) - mc), f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(bound<T>(m2, c) - mc);
+      const Base b = base_of<T>(m1, c);
+      const float f1 = m == -__builtin_inff() ? 0.f : ratio(b, base_of<T>(m, c), c), f2 = m2 == -__builtin_inff() ? 0.f : ratio(b, base_of<T>(m2, c), c);
       m = m1; l = l * f1 + l2 * f2;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -379,7 +401,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
     const long long n = (long long)a.rows_q * a.heads;
     if (live && kg == 0) {
       const long long pr = split * n + (long long)token * a.heads + head;
-      if (g == 0) { const sq_f2 x = {m == -__builtin_inff() ? m : bare<T>(bound<T>(m, c)), l * (1.f / Weight<T>::kTimes)}; *reinterpret_cast<sq_f2*>(a.ml + 2 * pr) = x; }
+      if (g == 0) { const sq_f2 x = {m, l}; *reinterpret_cast<sq_f2*>(a.ml + 2 * pr) = x; }
       float* op = a.part + pr * a.dim;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -401,8 +423,7 @@ seq_fwd_kernel(const SeqArgs a, const int tiles) {
       const int col = 32 * d + 8 * (i >> 2) + 4 * g;
       if (col < a.dim) seq_store4<T>(op + col, o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv, o[d][i + 3] * inv);
     }
-  // the weights are relative to the ROUNDED bound; what its rounding left belongs to the sum
-  if (a.lse && g == 0) a.lse[(long long)head * a.rows_q + token] = l != 0.f ? m * a.scale + (__logf(l * (1.f / Weight<T>::kTimes)) - kLn2 * __builtin_fmaf(m, c, -bare<T>(bound<T>(m, c)))) : -__builtin_inff();
+  if (a.lse && g == 0) a.lse[(long long)head * a.rows_q + token] = l != 0.f ? log_sum<T>(m, l, a.scale) : -__builtin_inff();
 }
 
 template <typename T>
