@@ -1173,3 +1173,32 @@ def test_logits_far_beyond_their_own_steps(eng, size, heads, kind):
             assert np.isfinite(got[:, h]).all()
             assert (np.abs(got[clear, h] - V[top[clear]]) <= 2 * u * np.abs(V[top[clear]]) + n * 1e-12).all()
     assert np.isfinite(lse.numpy()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [9, 10, 11, 12])
+def test_gradients_under_large_logits_stay_finite(eng, size, kind):
+    """P is formed anew from lse: with logits of up to 2^24 it may come out as some powers of two above 1, and has to have room for them."""
+    r = np.random.default_rng(size)
+    n, H, D = 400, 4, 128
+    q, k = (store(r.standard_normal((n, H, D)).clip(-3.9, 3.9) * 2.0 ** size, kind) for _ in range(2))
+    v, do = normal(r, kind, n, H, D), normal(r, kind, n, H, D)
+    q, k, v, do, c = (eng.to_device(x) for x in (q, k, v, do, starts([n])))
+    out, lse = sequence.packed_attention(eng, q, k, v, c)
+    for name, x in zip(("dq", "dk", "dv"), sequence.packed_attention_grad(eng, do, q, k, v, out, lse, c)):
+        got = value(x.numpy())
+        assert np.isfinite(got).mean() == 1 if name == "dv" or kind != "f16" else not np.isnan(got).any(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_gradients_of_rows_that_see_no_number_are_none(eng, kind):
+    r = np.random.default_rng(8)
+    n, H, D = 200, 2, 64
+    x = [normal(r, kind, n, H, D) for _ in range(4)]
+    x[1][100] = store(np.float32([np.nan]), kind)[0]
+    q, k, v, do, c = (eng.to_device(a) for a in (*x, starts([n])))
+    out, lse = sequence.packed_attention(eng, q, k, v, c)
+    dq, dk, dv = (value(a.numpy()) for a in sequence.packed_attention_grad(eng, do, q, k, v, out, lse, c))
+    assert np.isnan(dq[100:]).all() and np.isnan(dk).all() and np.isnan(dv).all()      # every key is seen by a row that sees key 100

@@ -8,7 +8,8 @@
 // form in 32 bits whose results are rounded once, dV within 1.4).  Every sum is held in 32 bits.
 // float16 holds 2^-24 .. 65504, dS anything (dout of 1e-4 over 2000 keys is below, dout of 1500 above): it is multiplied by a power of two
 // that fits the largest of its row (dQ) or key (dK) so far, a running bound as the forward's of the logits, and the sums are divided by it at the end.
-// P needs no such search, it is at most 1: 2^15 P goes into dV's product (weights below 2^-40 are lost, those from 2^-29 on are rounded like any other).
+// P needs no such search, it is at most 1 (and held there: under large logits the rounding of lse puts it above): 2^15 P goes into dV's product
+// (weights below 2^-40 are lost, those from 2^-29 on are rounded like any other).
 //
 // What bounds it: 4 sequences of up to 2048 rows, 32 heads over 8 of 128, bf16, causal: 256 us, 106 for dQ and 171 for dK and dV -- nine products
 // where the formulas have five, 0.79 PFLOP/s of them; a workgroup of dK and dV lasts as long as the rows that see its keys.  32 utterances of
@@ -334,7 +335,8 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * q + e;
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[e]));
+        float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[e]));
+        if constexpr (kFit) x = __builtin_elementwise_minimum(x, Weight<T>::kTimes);         // (NaN stays NaN)
         p[i] = x * (kFit ? __builtin_amdgcn_ldexpf(p[i] - de[e], lift) : p[i] - de[e]);
         s[i] = x;
       }
