@@ -252,10 +252,8 @@ __device__ __forceinline__ void seq_dma16(const void* base, unsigned offset, uns
 __device__ __forceinline__ void seq_dma4(const void* src, unsigned dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
 }
-// all but the newest `left` transfers have landed (a transfer lands in the order of its issue)
-template <int left = 0> __device__ __forceinline__ void seq_dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(left) : "memory"); }
-// every LDS read of the wave has been answered: what it read from may be overwritten
-__device__ __forceinline__ void seq_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// the wave's transfers have landed
+__device__ __forceinline__ void seq_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // The offsets of a wave's lanes in its transfers of 64 chunks (kRowsOf rows, `ld` bytes apart, ld a multiple of a tile's row): turn() of a sum of
 // rows without common bits is the exclusive or of their turns, and what a transfer's first row adds stays inside the row.  One register.
