@@ -259,7 +259,7 @@ int vnr_op_positional_encoding(vnr_handle h, int T, int dim, float step, float *
  * of 16 bytes.  scale > 0.  Outputs must not overlap inputs.  Rows outside d_cu[0] .. d_cu[batch] - 1 are neither read nor written, and a
  * masked or absent key contributes nothing whatever it holds (infinities and NaN included) -- see vnr_op_packed_attention_grad for its
  * exception.  Starts that run backwards make that sequence empty, starts outside the tensor count as its border -- for every operator alike --;
- * rows that more than one sequence then claims hold no defined values, nothing outside a tensor is touched.  Refused calls
+ * the rows of sequences that then overlap hold no defined values, nothing outside a tensor is touched.  Refused calls
  * return VNR_ERR_ARG with a message and launch nothing.  All calls are asynchronous on the handle's stream, which is not any other
  * library's: memory that another stream writes has to be complete before the call.  They look for no range word and raise none: one that
  * took results which VNR_ERR_RANGE voids is to be issued again like any other, over the same contents of d_context and d_table. */

@@ -4,16 +4,18 @@
 // workgroup that owns their keys): seq_dq_kernel goes over the keys of its query rows, seq_dkv_kernel over the query rows (of every head
 // of the group) of its keys.  Both rebuild S and dP -- seven products instead of the five that one pass with atomics onto dQ would take.
 // P is rounded once to the operands' type for dV (as dout is); what that rounding leaves of dS goes through a second product in 16-bit types --
-// the differences dP - delta cancel, and a rounding of what is left shows in dQ and dK (with it they are within 1.1 of the error of a plain
+// the differences dP - delta cancel, and a rounding of what is left shows in dQ and dK (with it they are within 1.01 of the error of a plain
 // form in 32 bits whose results are rounded once, dV within 1.4).  Every sum is held in 32 bits.
 // float16 holds 2^-24 .. 65504, dS anything (dout of 1e-4 over 2000 keys is below, dout of 1500 above): it is multiplied by a power of two
 // that fits the largest of its row (dQ) or key (dK) so far, a running bound as the forward's of the logits, and the sums are divided by it at the end.
 // P needs no such search, it is at most 1 (and held there: under large logits the rounding of lse puts it above): 2^15 P goes into dV's product
 // (weights below 2^-40 are lost, those from 2^-29 on are rounded like any other).
 //
-// What bounds it: 4 sequences of up to 2048 rows, 32 heads over 8 of 128, bf16, causal: 256 us, 106 for dQ and 171 for dK and dV -- nine products
-// where the formulas have five, 0.79 PFLOP/s of them; a workgroup of dK and dV lasts as long as the rows that see its keys.  32 utterances of
-// up to 400 rows, 4 heads of 64, f32: 113 us (52 + 66), the 32-bit matrix instructions' rate and LDS reads of four bytes a lane.
+// What bounds it: 4 sequences of up to 2048 rows, 32 heads over 8 of 128, bf16, causal: 254 - 265 us by card -- nine products where the formulas have
+// five, 0.79 PFLOP/s of them; a workgroup of dK and dV lasts as long as the rows that see its keys (the matrix pipe is busy 29 % of its cycles, 40 % of
+// dQ's).  32 utterances of up to 400 rows, 4 heads of 64, f32: 113 us, the 32-bit matrix instructions' rate (the pipe is busy 22 and 24 %: about one
+// wave a SIMD) and LDS reads of four bytes a lane.  (Under a profiler, which runs every kernel alone and at other clocks: 107 us for dQ and 171 for
+// dK and dV, 52 and 66.)
 #include "sequence.h"
 
 namespace vnr {
@@ -447,8 +449,9 @@ __global__ void __launch_bounds__(64 * KG * HG, HG == 4 || sizeof(T) * DP == 128
 
 // tiles of `rows` rows, at most: every sequence ends inside one
 long long tiles_of(int total, int batch, int rows) { return total / rows + (batch < total ? batch : total); }
-// Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 256 / 294 us
-// with four / two), two of them and twice the workgroups a unit where they pass few (the f32 case 124 / 113); rows of 512 bytes leave room for two
+// Four row groups where a sequence's first keys pass many tiles of rows (their workgroup outlasts the launch: the bf16 case above 255 / 291 us
+// with four / two), two of them and twice the workgroups a unit where they pass few (the f32 case 124 / 113, 8 sequences of up to 1000 192 / 174; the
+// border is crude: the bf16 case with sequences of up to 512 takes 64 / 73); rows of 512 bytes leave room for two
 int row_groups(const SeqArgs& f) {
   const long long turns = (long long)f.rows_q / f.batch * (f.heads / f.kv_heads) / 32;
   return (f.dtype == SEQ_F32 ? 4 : 2) * (f.dim <= 64 ? 64 : 128) <= 256 && turns >= 32 ? 4 : 2;
@@ -478,7 +481,7 @@ template <typename T, int DP> hipError_t grad(const SeqGradArgs& a, int cus, hip
   hipError_t e = hipSuccess;
   const SeqArgs& f = a.f;
   // 128 query rows a workgroup where that makes two for each compute unit, else 64 (32 utterances of up to 400 rows, 4 heads, f32: both kernels
-  // 135 / 113 us with 128 / 64; 4 sequences of up to 2048, 32 heads of 128, bf16: 256 / 269)
+  // 135 / 113 us with 128 / 64; 4 sequences of up to 512, 32 heads of 128, bf16: 78 / 73, of up to 2048: 256 / 269)
   const long long wgs = tiles_of(f.rows_q, f.batch, 128) * f.heads;
   if (f.rows_q > 0) e = wgs >= 2LL * cus ? grad_q<T, DP, 4, 1>(a, s) : grad_q<T, DP, 2, 2>(a, s);
   if (e != hipSuccess || f.rows_k == 0) return e;

@@ -1,6 +1,6 @@
 // New keys and values into a paged cache, turned by their positions on the way (and the queries of the same tokens beside them).
 // Bound by memory: every element is read once and written once, 16 bytes a lane (32 in 32 bits): prompts of 17555 rows in all, 32 + 8 heads of
-// 128, bf16: 84 us = 5.2 TB/s, as fast as a large copy; 8 rows 4.4 us, a launch and three loads that wait for each other (start, page, row).  One workgroup a token: the token's
+// 128, bf16: 84 us = 5.2 TB/s, as fast as a large copy; 8 rows 4.2 us, a launch and three loads that wait for each other (start, page, row).  One workgroup a token: the token's
 // angles stay in registers while a thread goes over its share of the heads.
 #include "sequence.h"
 

@@ -13,10 +13,10 @@
 // K and V tiles come straight from memory to LDS (16 bytes a lane, no registers), the next tile while this one is multiplied.
 //
 // What bounds it: long prompts the matrix pipe and the exponentials between its products (4 prompts of up to 4096 rows, 32 heads of 128, bf16, causal:
-// 417 us = 0.94 PFLOP/s of the products that are not masked; the pipe is busy 41 % of the time, its waves wait 43 %: for the barrier of a tile and
-// for each other's turns on the vector units); a decoding step memory (64 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16: 118 us =
-// 4.7 TB/s, 2 of 100000 keys 140 us = 5.5; a large copy reaches 5.0); few short sequences the way through one workgroup (4 utterances of up to
-// 101 rows: 9.6 us; the append of 8 rows, three loads that wait for each other and one store, takes 4.4).
+// 412 - 425 us by card = 0.96 - 0.93 PFLOP/s of the products that are not masked; 851 thousand cycles, 45 % of which the pipe is busy; the waves wait
+// 21 % of theirs for tiles and barriers and 35 % for each other's turns on the units); a decoding step memory (64 sequences of up to 4096 keys, 32
+// heads over 8 of 128, bf16: 117 us = 4.8 TB/s, 2 of 100000 keys 140 us = 5.5; a large copy reaches 5.0); few short sequences the way through one
+// workgroup (4 utterances of up to 101 rows: 10 us; the append of 8 rows, three loads that wait for each other and one store, takes 4.2).
 #include "sequence.h"
 
 namespace vnr {
@@ -472,9 +472,13 @@ long long join_grid(const SeqArgs& a) { return ((long long)a.rows_q * a.heads + 
 // Rows a workgroup.  Packed: 128 (every key tile is read once for them) where that makes two workgroups for each compute unit; else 64, else 32
 // with all four waves along the keys: a launch of few workgroups lasts as long as one of them (4 utterances of up to 101 rows, 4 heads, f32:
 // 15.8 / 11.1 / 9.8 us with 128 / 64 / 32 rows; 16 of up to 800, f16: 20.2 / 18.6 / 26.2; 4 prompts of up to 4096, 32 heads of 128, bf16:
-// 417 / 514 / 1138).  Over a cache: 64 rows where no sequence has more (group x new rows), else 128 (one row for each of 64 sequences:
-// 117.6 / 119.0 us with 64 / 128; chunks of up to 512: 250 / 182), and the keys are cut where the tiles alone leave compute units idle: two
-// workgroups for each of them, no piece shorter than 256 keys (1 row over 100000 keys, 2 sequences: 160 us with one for each, 138 with two).
+// 417 / 514 / 1138).  With the border at one workgroup for each unit, two and four: 32 utterances of up to 400, f32, 51.5 / 39.5 / 60.7; the 16,
+// 19.8 / 18.8 / 27.0; prompts of up to 400, bf16, 16.2 / 17.5 / 44.0.  Over a cache: 64 rows where no sequence has more (group x new rows), else 128
+// (one row for each of 64 sequences: 117.6 / 119.0 us with 64 / 128; chunks of up to 512: 250 / 182), and the keys are cut where the tiles alone leave
+// compute units idle: two workgroups for each of them (4 rows over 4096 keys: 22.5 us with one, 18.1 with two, 17.9 with four; 2 over 100000: 149 /
+// 143.5 / 150; chunks of 5 over 2000: 16.6 / 15.1 / 15.8), no piece shorter than 256 keys (1 row over 4096: 18.6 with 512, 15.3 with 256, 14.5 with
+// 128, over 1000 14.7 / 11.4 / 9.9; chunks of 5 16.5 / 15.1 / 15.2) and at most 64 pieces, one a lane of the join (1 row of one cache head over
+// 100000: 42.3 us, 67.8 with 32).
 SeqPlan seq_plan(const SeqArgs& a, int cus) {
   SeqPlan p;
   const int group = a.heads / a.kv_heads;
