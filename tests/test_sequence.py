@@ -1202,3 +1202,26 @@ def test_gradients_of_rows_that_see_no_number_are_none(eng, kind):
     out, lse = sequence.packed_attention(eng, q, k, v, c)
     dq, dk, dv = (value(a.numpy()) for a in sequence.packed_attention_grad(eng, do, q, k, v, out, lse, c))
     assert np.isnan(dq[100:]).all() and np.isnan(dk).all() and np.isnan(dv).all()      # every key is seen by a row that sees key 100
+
+
+def test_cache_calls_behind_fills_do_not_wait_for_the_device(monkeypatch):
+    """Zeroed or random arrays raise no range word: calls on them go out at once, and a later replay does not lay the fills over their results."""
+    lib = Script("vnr_prior_sample")
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    e = _lib.Engine.__new__(_lib.Engine)
+    e.lib, e.handle, e._log, e._log_cap, e._training_mode, e.range_replays = lib, 1, [], 256, False, 0
+    e._pool, e._pool_bytes, e._pool_cap = {}, 0, 1 << 30
+    array = lambda shape, kind=np.float16: _lib.DeviceArray(e, shape, kind, ptr=4096, owner=lib)
+    q, cu, ctx, table = array((6, 4, 64)), array((3,), np.int32), array((2,), np.int32), array((2, 3), np.int32)
+    cache = sequence.PagedCache(e, array((4, 2, 16, 64)), array((4, 2, 16, 64)))
+    e.set_option("n_sample", 1)
+    for _ in range(3):
+        e.call("vnr_memset", 4096, 0, 64)
+        e.call("vnr_random_normal", 1, 0, 1.0, 4096, 16)
+        cache.attend(q, cu, ctx, table, 1, 40, out=q)
+    assert lib.calls == ["vnr_set_option"] + ["vnr_memset", "vnr_random_normal", "vnr_op_paged_attention"] * 3
+    lib.calls.clear()
+    e.call("vnr_prior_sample")
+    e.synchronize()
+    assert lib.calls == ["vnr_prior_sample", "vnr_synchronize", "vnr_set_option", "vnr_prior_sample", "vnr_synchronize"]
+    e.handle = None

@@ -365,9 +365,12 @@ class Engine:
 
     def call_once(self, name, *args):
         """An entry point that is never issued again: its arrays may be another library's, which may have freed or rewritten them by the time
-        of a replay.  What is pending is settled first (a synchronisation, and the replay if the word is raised); the call itself is not recorded."""
-        if self._pending():
+        of a replay.  What is pending is settled first (a synchronisation, and the replay if the word is raised); the call itself is not recorded.
+        Fills cannot raise the word: alone in the log they are settled as they are, and leave it -- a replay would lay them over this call's results."""
+        if any(name not in ("vnr_set_option", "vnr_memset", "vnr_random_normal") for name, _ in self._log):
             self.synchronize()
+        elif self._log:
+            self._log = [entry for entry in self._log if entry[0] == "vnr_set_option"]
         self.call(name, *args, record=False)
 
     def _pending(self):
