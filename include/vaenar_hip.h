@@ -254,7 +254,7 @@ int vnr_op_positional_encoding(vnr_handle h, int T, int dim, float step, float *
  * Ragged batches without their padding: the rows of all sequences lie one behind the other in [rows][heads][head_dim] matrices (a row
  * stride in ELEMENTS may leave room between rows: column blocks of one projection), sequence b owning rows d_cu[b] .. d_cu[b + 1] - 1
  * (device int32 [batch + 1], ascending).  Query head h reads key / value head h / (heads / kv_heads).  Types: every tensor of a call in the
- * same one of the three; products are rounded once (16 bits: the probabilities and their gradients as operands of the second products),
+ * same one of the three; products are rounded once (16 bits: the probabilities and their gradients as operands of the second products; float16: of a weight by 2^-36 of its row's largest),
  * maxima, sums and accumulators are 32 bits.  head_dim: a multiple of 8, at most 128.  Matrices: 16-byte aligned, row strides a multiple
  * of 16 bytes.  scale > 0.  Outputs must not overlap inputs.  Rows outside d_cu[0] .. d_cu[batch] - 1 are neither read nor written, and a
  * masked or absent key contributes nothing whatever it holds (infinities and NaN included) -- see vnr_op_packed_attention_grad for its

@@ -35,7 +35,7 @@ struct SeqGradArgs {
   SeqArgs f;
   const void* dout = nullptr; long long lddo = 0;
   void *dq = nullptr, *dk = nullptr, *dv = nullptr; long long lddq = 0, lddk = 0, lddv = 0;
-  float* delta = nullptr;                                            // [heads][rows_q] scratch: sum_d dout * out of every row
+  float* delta = nullptr;                                            // [2][heads][rows_q] scratch: sum_d dout * out of every row; its lse in units of log2, less the lift of the weights
 };
 hipError_t launch_seq_grad(const SeqGradArgs& a, int compute_units, hipStream_t s);
 
